@@ -9,19 +9,30 @@ if the CUDA library is missing.
 """
 from .bridge import (  # noqa: F401
     install,
+    load_mac_chunk_attention_extension,
     load_mac_decode_rope_preserve_extension,
     load_mac_merge_downdate_cache_extension,
     load_mac_persistent_decode_extension,
     load_mac_prefill_update_cache_extension,
+    load_mac_quantized_cache_extension,
 )
-from .workspace import make_decision_workspace, make_decode_workspace  # noqa: F401
+from .workspace import (  # noqa: F401
+    make_chunk_attention_workspace,
+    make_decision_workspace,
+    make_decode_workspace,
+    make_quantized_pool,
+)
 
 __all__ = [
     "install",
+    "load_mac_chunk_attention_extension",
     "load_mac_decode_rope_preserve_extension",
     "load_mac_merge_downdate_cache_extension",
     "load_mac_persistent_decode_extension",
     "load_mac_prefill_update_cache_extension",
+    "load_mac_quantized_cache_extension",
+    "make_chunk_attention_workspace",
     "make_decision_workspace",
     "make_decode_workspace",
+    "make_quantized_pool",
 ]

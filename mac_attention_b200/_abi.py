@@ -1,4 +1,4 @@
-"""ctypes view of ``include/mac_b200.h`` and the library loader."""
+"""ctypes view of ``include/mac_b200.h`` and ``include/mac_b200_chunk.h``, and the library loader."""
 from __future__ import annotations
 
 import ctypes as C
@@ -105,6 +105,49 @@ PROTOTYPES = {
     "mac_b200_selftest_bounded_wait": (C.c_int, [C.POINTER(C.c_uint32), C.POINTER(C.c_int32), ptr]),
 }
 
+
+class MacB200ChunkArgs(C.Structure):
+    _fields_ = [
+        ("B", i32), ("Hq", i32), ("Hkv", i32), ("D", i32), ("q_rows", i32),
+        ("req_to_token_rows", i32), ("req_to_token_stride", i32), ("window", i32),
+        ("kv_tokens", i64), ("q_stride0", i64), ("workspace_bytes", i64),
+        ("sm_scale", f32), ("reserved", i32),
+        ("q", ptr), ("k", ptr), ("v", ptr), ("k_exp", ptr), ("v_exp", ptr),
+        ("req_to_token", ptr), ("req_ids", ptr), ("offsets", ptr), ("kv_lens", ptr),
+        ("out", ptr), ("lse", ptr), ("workspace", ptr),
+    ]
+
+
+class MacB200QuantizeKvArgs(C.Structure):
+    _fields_ = [
+        ("N", i64), ("Hq", i32), ("Hkv", i32), ("D", i32), ("cache_locs_i64", i32),
+        ("k_stride0", i64), ("v_stride0", i64), ("kv_pool_tokens", i64),
+        ("k", ptr), ("v", ptr), ("k_pool", ptr), ("v_pool", ptr), ("k_exp", ptr), ("v_exp", ptr),
+        ("cache_locs", ptr),
+        ("q", ptr), ("q_post", ptr), ("cos_sin_cache", ptr), ("positions", ptr),
+        ("q_stride0", i64), ("cos_sin_stride0", i64), ("max_positions", i64),
+        ("rotary_dim", i32), ("is_neox", i32), ("positions_i64", i32), ("reserved", i32),
+    ]
+
+
+class MacB200DequantizeKvArgs(C.Structure):
+    _fields_ = [
+        ("N", i64), ("Hkv", i32), ("D", i32), ("src_locs_i64", i32), ("dst_locs_i64", i32),
+        ("src_tokens", i64), ("dst_tokens", i64),
+        ("k_pool", ptr), ("v_pool", ptr), ("k_exp", ptr), ("v_exp", ptr), ("src_locs", ptr),
+        ("k_buffer", ptr), ("v_buffer", ptr), ("dst_locs", ptr),
+    ]
+
+
+# The same for include/mac_b200_chunk.h.
+CHUNK_PROTOTYPES = {
+    "mac_b200_chunk_attention_bf16": (C.c_int, [C.POINTER(MacB200ChunkArgs), ptr]),
+    "mac_b200_chunk_attention_e4m3": (C.c_int, [C.POINTER(MacB200ChunkArgs), ptr]),
+    "mac_b200_chunk_attention_workspace_bytes": (C.c_int, [C.POINTER(C.c_int64)]),
+    "mac_b200_quantize_kv_e4m3": (C.c_int, [C.POINTER(MacB200QuantizeKvArgs), ptr]),
+    "mac_b200_dequantize_kv_e4m3": (C.c_int, [C.POINTER(MacB200DequantizeKvArgs), ptr]),
+}
+
 ABI_VERSION = 2
 _lib = None
 
@@ -136,7 +179,7 @@ def load_library() -> C.CDLL:
     if not path.exists():
         raise RuntimeError(f"CUDA library not found: {path}")
     lib = C.CDLL(str(path))
-    for name, (res, args) in PROTOTYPES.items():
+    for name, (res, args) in {**PROTOTYPES, **CHUNK_PROTOTYPES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -68,6 +68,34 @@ def load_mac_merge_downdate_cache_extension(verbose: bool = False) -> Any:
         mac_update_then_downdate_bf16_inplace=ops.mac_update_then_downdate_bf16_inplace)
 
 
+@lru_cache(maxsize=1)
+def load_mac_chunk_attention_extension(verbose: bool = False) -> Any:
+    """Attention of a chunk of new tokens over the paged pool (no loader of the reference
+    has it: there, prompt attention comes from another library)."""
+    _abi.load_library()
+    from . import ops
+
+    return SimpleNamespace(
+        mac_chunk_attention_bf16=ops.mac_chunk_attention_bf16,
+        mac_chunk_attention_e4m3=ops.mac_chunk_attention_e4m3,
+        query_status=ops.query_status,
+    )
+
+
+@lru_cache(maxsize=1)
+def load_mac_quantized_cache_extension(verbose: bool = False) -> Any:
+    """Writing and reading back rows of an 8-bit K/V pool (not in the reference)."""
+    _abi.load_library()
+    from . import ops
+
+    return SimpleNamespace(
+        mac_quantize_kv_e4m3=ops.mac_quantize_kv_e4m3,
+        mac_decode_rope_quantize_kv_e4m3=ops.mac_decode_rope_quantize_kv_e4m3,
+        mac_dequantize_kv_e4m3=ops.mac_dequantize_kv_e4m3,
+        query_status=ops.query_status,
+    )
+
+
 _PATCHED = ("load_mac_persistent_decode_extension", "load_mac_prefill_update_cache_extension",
             "load_mac_decode_rope_preserve_extension", "load_mac_merge_downdate_cache_extension")
 _HOOK_MODULES = (

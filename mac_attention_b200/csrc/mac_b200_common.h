@@ -31,6 +31,10 @@ int take_prefill_build_status(unsigned* bits);
 // The same for the tensor-memory variant of the sink-exclusive build.
 int take_prefill_sink_tc_status(unsigned* bits);
 
+// The same for the chunk attention and for the 8-bit pool's write and read kernels.
+int take_chunk_status(unsigned* bits);
+int take_kv8_status(unsigned* bits);
+
 // Sink-exclusive prefill build on tcgen05 / tensor memory (validated arguments); sets
 // *launched when it ran, leaves it false when this step has to take the mma.sync kernel.
 int launch_prefill_sink_exclusive_tc(const ::MacB200PrefillBuildArgs& a, int sms, cudaStream_t stream,

@@ -2430,7 +2430,10 @@ extern "C" int mac_b200_query_status(uint32_t* status_out, void* stream_v) {
   MAC_CUDA(cudaMemcpyFromSymbol(&v, g_status, sizeof(v)));
   unsigned build_bits = 0;
   if (const int rc = take_prefill_build_status(&build_bits)) return rc;
-  *status_out = v | build_bits;
+  unsigned chunk_bits = 0, kv8_bits = 0;
+  if (const int rc = take_chunk_status(&chunk_bits)) return rc;
+  if (const int rc = take_kv8_status(&kv8_bits)) return rc;
+  *status_out = v | build_bits | chunk_bits | kv8_bits;
   if (v != 0) {
     const unsigned zero = 0;
     MAC_CUDA(cudaDeviceSynchronize());

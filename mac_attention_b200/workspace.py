@@ -69,3 +69,31 @@ def make_decision_workspace(batch, hq, hkv, capacity, match_tile_slots, *, devic
         torch.empty(9, **i32),
         torch.zeros(phase_slots, device=device, dtype=torch.int64),
     ]
+
+
+def make_chunk_attention_workspace(device="cuda"):
+    """The scratch of ``mac_chunk_attention_bf16`` / ``_e4m3``: split results and arrival
+    counters, whatever the sizes of the calls.  Its size depends on the device alone; it is
+    zeroed here once and every call leaves its counters at zero.  Calls that may overlap on
+    the device (two streams, two graphs replayed side by side) need one each; calls in order
+    share one."""
+    import ctypes as C
+
+    from . import _abi
+
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise RuntimeError("the chunk attention workspace lives on a CUDA device")
+    n = C.c_int64(0)
+    with torch.cuda.device(dev):
+        _abi.check(_abi.load_library().mac_b200_chunk_attention_workspace_bytes(C.byref(n)))
+        return torch.zeros(n.value, dtype=torch.uint8, device=dev)
+
+
+def make_quantized_pool(tokens, hkv, *, device="cuda"):
+    """An empty 8-bit pool of ``tokens`` rows: ``(k_pool, v_pool, k_exp, v_exp)``, e4m3 codes
+    ``[tokens, hkv, 128]`` and one exponent byte per row ``[tokens, hkv]`` (rows of zeros)."""
+    pools = [torch.zeros(tokens, hkv, 128, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    exps = [torch.full((tokens, hkv), 3, dtype=torch.uint8, device=device) for _ in range(2)]
+    return (*pools, *exps)
