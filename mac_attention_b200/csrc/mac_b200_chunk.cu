@@ -1,7 +1,35 @@
 // Attention of a chunk of new tokens over the paged K/V pool, bf16 or e4m3 (sm_100a).
 // Semantics: include/mac_b200_chunk.h.
+//
+// Rows.  A KV head's G query heads see the same keys, so the rows of a tile are (token, query
+// head) pairs: 128/G tokens x G heads fill the 128 rows of a tcgen05 product.  A UNIT of work is
+// (request, KV head, up to two tiles of rows) with the keys that its rows attend together, in
+// blocks of 128 keys.  Two tiles ("dual") share every staged K/V block, which halves the traffic
+// through shared memory; a unit whose rows fit one tile ("single": decode, drafted tokens, a
+// prompt's remainder) lets its two softmax streams take alternate blocks of the same rows and
+// joins the two results at the end.  Either way two streams are in flight, and while one is in its
+// softmax the other's products run.
+//
+// Split.  All blocks of all units lie on one line (request, KV head, tile, block) that is cut into
+// equal parts, one per CTA: no tail wave whatever the lengths.  A unit that a cut falls into
+// leaves unnormalised partial results (fp32) in the workspace, and the CTA that arrives last joins
+// them in the order of the parts, so the result does not depend on timing.  Every CTA works its
+// part out from the lengths by itself; there is no planning launch, and no CTA waits for another.
+//
+// Roles of a CTA (one per SM):
+//   warps 0-3 / 4-7  softmax streams 0 / 1, one thread per row: scores from tensor memory, running
+//                    maximum and sum in fp32, bf16 weights back over the scores, results out
+//   warp 8           issues the products: S = Q K^T from shared memory, O += P V with P read from
+//                    tensor memory and V from the rows as they lie in the pool (keys x dims)
+//   warps 9, 11      fetch K/V rows by the page table into the swizzled operand layout (cp.async)
+//   warp 10          works out the units of this CTA's part, fetches the query tiles
+// The running maximum is kept until a row's scores exceed it by 2^8 in weight: the rescaling of O
+// is rare, and exact when it happens.  Weights are rounded to bf16 for the second product (the
+// operand type); the sum of weights is taken before that rounding, in fp32.
+#include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <climits>
 #include <cmath>
 
 #include "mac_b200_common.h"
@@ -12,15 +40,867 @@
 namespace mac_b200 {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kBlk = 128;                  // keys of a block
+constexpr int kRows = 128;                 // rows of a tile
+constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 bf16 in the 128-byte-swizzled layout
+constexpr int kTileBytes = 2 * kHalfBytes;
+constexpr int kStages = 5;                 // K/V blocks in shared memory
+constexpr int kItems = 4;                  // units announced ahead
+constexpr int kSoftmaxWarps = 8;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;
+constexpr int kThreads = 384;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // 256 * 216 + 128 * 72 = 384 * 168
+constexpr int kMinBlocks = 4;              // fewest blocks worth a CTA of their own
+constexpr int kTmemCols = 512;             // S0 S1 O0 O1; the weights lie over the scores
+constexpr int kRowWarps = 8;
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+
+// A slot of the workspace: one part's unnormalised results, two streams of 128 rows.
+constexpr int64_t kSlotFloats = 2 * kRows * 128;
+constexpr int64_t kSlotBytes = kSlotFloats * 4 + 2 * kRows * 8;
+
+// bf16 x bf16 -> fp32, M 128, N 128; the second product's B operand is dim-contiguous
+constexpr uint32_t kIdescQk = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescPv = kIdescQk | (1u << 16);
 
 __device__ unsigned g_chunk_status = 0;
 
+struct Item {
+  int valid, dual;
+  int kh, req;             // KV head, row of the page table
+  int tok0, ntok;          // first row of q, tokens
+  int pos0;                // position of the first token (negative: attends nothing)
+  int k0, khi;             // keys [k0, khi) are attended by some row of the unit
+  int blk0, nblk;          // this part's blocks, counted from k0
+  int qbuf;                // query buffer of a single unit
+  int parts, cta0;         // CTAs that share the unit, the first of them
+  int slot;
+  unsigned nonfinite;      // a value that only some rows attend was infinite or NaN
+};
+
+struct Control {
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  uint64_t item_full[kItems], item_empty[kItems], join;
+  Item items[kItems];
+  long long scan[kThreads / 32];
+  long long start_pos;     // where request start_b begins on the line
+  int start_b;
+  uint32_t tmem;
+  unsigned abort;
+  unsigned last;
+};
+
+constexpr int kSmemQ = 0;
+constexpr int kSmemKv = 2 * kTileBytes;
+constexpr int kSmemControl = kSmemKv + kStages * kTileBytes;
+constexpr int kSmemBytes = kSmemControl + static_cast<int>(sizeof(Control)) + 1024;   // + alignment
+static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits for the phase of `count` earlier phases.  False when the limit ran out here or in another
+// warp of the CTA: the caller leaves its loop.
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, unsigned* abort_flag) {
+  const unsigned long long t0 = now_ns();
+  for (unsigned spins = 1;; ++spins) {
+    if (mbar_try(bar, parity)) return true;            // each try may itself block for a while
+    if ((spins & 31u) == 0u) {
+      if (*reinterpret_cast<volatile unsigned*>(abort_flag) != 0u) return false;
+      if (now_ns() - t0 > kWaitLimitNs) {
+        *reinterpret_cast<volatile unsigned*>(abort_flag) = 1u;
+        atomicOr(&g_chunk_status, MAC_B200_STATUS_COPY_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned* abort_flag) {
+  const uint32_t b = smem_u32(bar);
+  if (mbar_try(b, parity & 1u)) return true;
+  return mbar_wait_slow(b, parity & 1u, abort_flag);
+}
+
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// Operand in shared memory, 128-byte swizzle, eight-row groups 1024 bytes apart.  `lead`: bytes
+// between the two 64-dim halves when the operand is dim-contiguous (unused when key-contiguous).
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead) {
+  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+         (static_cast<uint64_t>(2) << 61);
+}
+// D (+)= A B^T, 128 x 128 x 16: A and B from shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(kIdescQk), "r"(accumulate)
+      : "memory");
+}
+// D (+)= A B, 128 x 128 x 16: A from tensor memory, B dim-contiguous from shared memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(kIdescPv), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_u32(bar))
+               : "memory");
+}
+// 32 consecutive columns of this thread's tensor-memory lane; tmem_ld_wait() before they are used
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_wait() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+// 16 bytes, or 16 zeros when `bytes` is 0
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// arrives on `bar` once this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// rows written by cp.async (or by stores) that a barrier has made visible here, to the copy
+// engine's and the tensor cores' view of shared memory
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// ---------------------------------------------------------------------------- units on the line
+struct Request {
+  int row0, n, kv, req;
+};
+// `report`: set the status bit for what cannot be run (one thread of the grid does)
+__device__ __forceinline__ Request load_request(const MacB200ChunkArgs& a, int b, bool report) {
+  Request r;
+  const int o0 = a.offsets[b], o1 = a.offsets[b + 1];
+  r.row0 = o0;
+  r.n = o1 - o0;
+  r.req = a.req_ids[b];
+  r.kv = a.kv_lens[b];
+  bool bad = false;
+  if (o0 < 0 || o1 < o0 || o1 > a.q_rows) {
+    r.n = 0;
+    bad = true;
+  } else if (r.req < 0 || r.req >= a.req_to_token_rows || r.kv < 0 || r.kv > a.req_to_token_stride) {
+    r.kv = 0;                                            // rows without keys
+    r.req = 0;
+    bad = true;
+  }
+  if (bad && report) atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+  return r;
+}
+struct Unit {
+  int t0, ntok;            // tokens of the request
+  int k0, khi, nblk;
+};
+__device__ __forceinline__ Unit unit_of(const Request& r, int window, int tile_tokens, int t) {
+  Unit u;
+  u.t0 = t * 2 * tile_tokens;
+  u.ntok = min(2 * tile_tokens, r.n - u.t0);
+  const int p0 = r.kv - r.n + u.t0;
+  u.khi = max(0, p0 + u.ntok);
+  u.k0 = 0;
+  if (window >= 0) u.k0 = static_cast<int>(max(0ll, static_cast<long long>(p0) + 1 - window));
+  u.nblk = window == 0 || u.k0 >= u.khi ? 0 : (u.khi - u.k0 + kBlk - 1) / kBlk;
+  return u;
+}
+__device__ __forceinline__ int units_of(const Request& r, int tile_tokens) {
+  return (r.n + 2 * tile_tokens - 1) / (2 * tile_tokens);
+}
+// length of one KV head of a request on the line: its blocks, 1 for a unit without keys
+__device__ __forceinline__ long long head_length(const Request& r, int window, int tile_tokens) {
+  long long c = 0;
+  const int nt = units_of(r, tile_tokens);
+  for (int t = 0; t < nt; ++t) c += max(1, unit_of(r, window, tile_tokens, t).nblk);
+  return c;
+}
+
+// The ring position of block `blk`'s K and V within a unit: K and V in turn when both streams use
+// each block; one K ahead when the streams alternate (K0 K1 V0 K2 V1 ...).
+__device__ __forceinline__ int ring_k(int dual, int blk) { return dual ? 2 * blk : (blk == 0 ? 0 : 2 * blk - 1); }
+__device__ __forceinline__ int ring_v(int dual, int blk, int nblk) {
+  return dual ? 2 * blk + 1 : min(2 * blk + 2, 2 * nblk - 1);
+}
+// and back: what ring position i holds
+__device__ __forceinline__ void ring_at(int dual, int nblk, int i, int& blk, bool& is_v) {
+  if (dual) {
+    blk = i >> 1;
+    is_v = i & 1;
+  } else if (i == 0) {
+    blk = 0;
+    is_v = false;
+  } else if (i & 1) {
+    blk = (i + 1) >> 1;
+    is_v = blk >= nblk;
+    if (is_v) blk = nblk - 1;
+  } else {
+    blk = (i - 2) >> 1;
+    is_v = true;
+  }
+}
+
+// Whether some row of the unit attends only a part of the keys of block [kb, kb + 128) that exist.
+__device__ __forceinline__ bool partly_attended(const Item& it, int window, int kb) {
+  const int last = it.pos0 + it.ntok - 1;
+  return min(kb + kBlk, it.khi) > it.pos0 + 1 ||
+         (window >= 0 && static_cast<long long>(kb) < static_cast<long long>(last) + 1 - window);
+}
+
+__device__ __forceinline__ const void* v_row(const MacB200ChunkArgs& a, const Item& it, int key) {
+  const int tok = a.req_to_token[static_cast<int64_t>(it.req) * a.req_to_token_stride + key];
+  if (tok < 0 || tok >= a.kv_tokens) return nullptr;
+  return static_cast<const char*>(a.v) + (static_cast<int64_t>(tok) * a.Hkv + it.kh) * 256;
+}
+
+// ------------------------------------------------------------------------------------ the kernel
+__global__ void __launch_bounds__(kThreads, 1)
+chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtensorMap q_map) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  Control& ctl = *reinterpret_cast<Control*>(smem + kSmemControl);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.Hq / a.Hkv;
+  const int tile_tokens = kRows / G;
+
+  // ---- the line: this CTA's part of it, and the request that the part begins in
+  const int per = (a.B + kThreads - 1) / kThreads;
+  const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b)
+    mine += a.Hkv * head_length(load_request(a, b, blockIdx.x == 0), a.window, tile_tokens);
+  long long before = mine;                               // inclusive within the warp, then exclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += o;
+  }
+  if (lane == 31) ctl.scan[warp] = before;
+  __syncthreads();
+  long long total = 0;
+  before -= mine;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += ctl.scan[w];
+    total += ctl.scan[w];
+  }
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1ll, total / kMinBlocks)));
+  if (total == 0 || static_cast<int>(blockIdx.x) >= ctas) return;
+  const long long lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
+  if (lo >= before && lo < before + mine) {
+    long long at = before;
+    for (int b = b0; b < b1; ++b) {
+      const long long len = a.Hkv * head_length(load_request(a, b, false), a.window, tile_tokens);
+      if (lo < at + len) {
+        ctl.start_b = b;
+        ctl.start_pos = at;
+        break;
+      }
+      at += len;
+    }
+  }
+
+  // ---- barriers, tensor memory
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&ctl.kv_full[i], 64);
+      mbar_init(&ctl.kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl.q_full[i], 1);
+      mbar_init(&ctl.q_empty[i], 1);
+      mbar_init(&ctl.s_full[i], 1);
+      mbar_init(&ctl.p_full[i], 4);
+      mbar_init(&ctl.o_full[i], 1);
+    }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&ctl.item_full[i], 1);
+      mbar_init(&ctl.item_empty[i], kSoftmaxWarps + 3);
+    }
+    mbar_init(&ctl.join, kSoftmaxWarps);
+    ctl.abort = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl.tmem;
+  unsigned* const abort_flag = &ctl.abort;
+
+  if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+
+    if (warp == kPlanWarp && lane == 0) {
+      // ---- the units of this part, in order, and their query tiles
+      long long cur = lo, req_pos = ctl.start_pos;
+      int b = ctl.start_b, it = 0, toggle = 0;
+      uint32_t q_uses[2] = {0u, 0u};
+      bool ok = true;
+      const uint32_t q_bytes = static_cast<uint32_t>(tile_tokens) * G * 128u;   // of one 64-dim half
+      while (ok && cur < hi) {
+        const Request r = load_request(a, b, false);
+        const long long len = r.n > 0 ? head_length(r, a.window, tile_tokens) : 0;
+        if (cur >= req_pos + len * a.Hkv) {
+          req_pos += len * a.Hkv;
+          ++b;
+          continue;
+        }
+        int kh = static_cast<int>((cur - req_pos) / len), t = 0;
+        long long u0 = req_pos + kh * len;
+        Unit u = unit_of(r, a.window, tile_tokens, 0);
+        while (cur >= u0 + max(1, u.nblk)) {
+          u0 += max(1, u.nblk);
+          u = unit_of(r, a.window, tile_tokens, ++t);
+        }
+        const int nt = units_of(r, tile_tokens);
+        while (ok && cur < hi && kh < a.Hkv) {
+          const long long u1 = u0 + max(1, u.nblk);
+          const long long end = min(hi, u1);
+          const int slot = it & (kItems - 1);
+          ok = ok && mbar_wait(&ctl.item_empty[slot], (it / kItems) + 1, abort_flag);
+          if (!ok) break;
+          Item& o = ctl.items[slot];
+          o.valid = 1;
+          o.dual = u.ntok > tile_tokens;
+          o.kh = kh;
+          o.req = r.req;
+          o.tok0 = r.row0 + u.t0;
+          o.ntok = u.ntok;
+          o.pos0 = r.kv - r.n + u.t0;
+          o.k0 = u.k0;
+          o.khi = u.khi;
+          o.blk0 = static_cast<int>(cur - u0);
+          o.nblk = u.nblk == 0 ? 0 : static_cast<int>(end - cur);
+          o.qbuf = toggle;
+          o.cta0 = static_cast<int>(((u0 + 1) * ctas - 1) / total);
+          o.parts = static_cast<int>((u1 * ctas - 1) / total) - o.cta0 + 1;
+          o.slot = 2 * static_cast<int>(blockIdx.x) + (o.cta0 == static_cast<int>(blockIdx.x) ? 1 : 0);
+          o.nonfinite = 0u;
+          const int dual = o.dual, tok0 = o.tok0, nblk = o.nblk;
+          mbar_arrive(&ctl.item_full[slot]);
+          if (nblk > 0) {
+            for (int i = 0; i < (dual ? 2 : 1) && ok; ++i) {
+              const int buf = dual ? i : toggle;
+              ok = mbar_wait(&ctl.q_empty[buf], q_uses[buf] + 1, abort_flag);
+              if (!ok) break;
+              ++q_uses[buf];
+              mbar_expect_tx(&ctl.q_full[buf], 2 * q_bytes);
+              const uint32_t dst = smem_u32(smem + kSmemQ + buf * kTileBytes);
+              tma_load_3d(dst, &q_map, 0, kh * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
+              tma_load_3d(dst + kHalfBytes, &q_map, 64, kh * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
+            }
+            if (!dual) toggle ^= 1;
+          }
+          ++it;
+          cur = end;
+          u0 = u1;
+          if (++t == nt) {
+            t = 0;
+            ++kh;
+          }
+          u = unit_of(r, a.window, tile_tokens, t);
+        }
+      }
+      const int slot = it & (kItems - 1);
+      if (ok && mbar_wait(&ctl.item_empty[slot], (it / kItems) + 1, abort_flag)) {
+        ctl.items[slot].valid = 0;
+        mbar_arrive(&ctl.item_full[slot]);
+      }
+      // a query tile still on its way when the CTA gives up must land before the CTA leaves
+      if (*reinterpret_cast<volatile unsigned*>(abort_flag) != 0u)
+        for (int i = 0; i < 2; ++i) {
+          const unsigned long long t0 = now_ns();
+          while (q_uses[i] > 0 && !mbar_try(smem_u32(&ctl.q_full[i]), (q_uses[i] - 1) & 1u) &&
+                 now_ns() - t0 < kWaitLimitNs) {}
+        }
+    } else if (warp == kLoadWarp || warp == kLoadWarp + 2) {
+      // ---- K/V rows by the page table: sixteen lanes fetch a row, a warp 64 of a block's 128
+      const int half = warp == kLoadWarp ? 0 : 64;
+      const int sub = lane >> 4, chunk = lane & 15;
+      const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 256;
+      uint32_t to[4];                                    // where this lane's chunk goes in rows 2i + sub
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = half + 2 * i + sub;
+        to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
+                (((chunk & 7) ^ (row & 7)) << 4);
+      }
+      uint32_t pos = 0;
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        const int slot = it & (kItems - 1);
+        ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const Item& o = ctl.items[slot];
+        if (!o.valid) break;
+        const int dual = o.dual, nblk = o.nblk, khi = o.khi;
+        const int first = o.k0 + o.blk0 * kBlk;
+        const int64_t col = o.kh * 256 + chunk * 16;
+        const int32_t* table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
+        // pool rows of keys `lane` and 32 + `lane` of this warp's half; -1: no key, arrives as zeros
+        auto rows_of = [&](int i, int (&row)[2], bool& is_v) {
+          int blk;
+          ring_at(dual, nblk, i, blk, is_v);
+          const int key = first + blk * kBlk + half + lane;
+          row[0] = key < khi ? __ldg(table + key) : -1;
+          row[1] = key + 32 < khi ? __ldg(table + key + 32) : -1;
+          return key;
+        };
+        int next[2] = {-1, -1};
+        bool next_v = false;
+        int next_key = nblk > 0 ? rows_of(0, next, next_v) : 0;
+        for (int i = 0; i < 2 * nblk; ++i, ++pos) {
+          int row[2] = {next[0], next[1]};
+          const bool is_v = next_v;
+          const int key = next_key;
+          if (i + 1 < 2 * nblk) next_key = rows_of(i + 1, next, next_v);
+          bool bad = false;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (key + 32 * j < khi && (row[j] < 0 || row[j] >= a.kv_tokens)) {
+              bad = true;
+              row[j] = -1;
+            }
+          if (bad) atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+          const int st = pos % kStages;
+          ok = mbar_wait(&ctl.kv_empty[st], pos / kStages + 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const char* src = static_cast<const char*>(is_v ? a.v : a.k) + col;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int tok = __shfl_sync(0xffffffffu, row[j >> 4], (2 * j & 31) + sub);
+            cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes,
+                       src + (tok < 0 ? 0 : tok) * row_stride, tok < 0 ? 0 : 16);
+          }
+          cp_async_arrive(&ctl.kv_full[st]);
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");   // nothing in flight when the CTA leaves
+    } else if (warp == kMmaWarp && lane == 0) {
+      // ---- products
+      uint32_t pos = 0, q_uses[2] = {0u, 0u}, p_uses[2] = {0u, 0u};
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        const int slot = it & (kItems - 1);
+        if (!mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag)) break;
+        const Item& o = ctl.items[slot];
+        if (!o.valid) break;
+        const int dual = o.dual, nblk = o.nblk, qbuf = o.qbuf;
+        mbar_arrive(&ctl.item_empty[slot]);
+        const int n = dual ? 2 * nblk : nblk;            // steps; stream = step & 1
+        auto scores = [&](int i) {                       // S[stream] = Q K^T
+          const int s = i & 1, blk = dual ? i >> 1 : i, buf = dual ? s : qbuf;
+          if (dual ? i < 2 : i == 0) {
+            if (!mbar_wait(&ctl.q_full[buf], q_uses[buf], abort_flag)) return false;
+            ++q_uses[buf];
+          }
+          const uint32_t p = pos + ring_k(dual, blk), st = p % kStages;
+          if (!mbar_wait(&ctl.kv_full[st], p / kStages, abort_flag)) return false;
+          fence_async_smem();
+          tc_fence_after();
+          const uint64_t dq = operand_desc(smem_u32(smem + kSmemQ + buf * kTileBytes), 16);
+          const uint64_t dk = operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes), 16);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
+            mma_ss(tmem + s * 128, dq + off, dk + off, k > 0);
+          }
+          mma_commit(&ctl.s_full[s]);
+          if (!dual || s == 1) mma_commit(&ctl.kv_empty[st]);
+          if (dual ? blk == nblk - 1 : i == n - 1) mma_commit(&ctl.q_empty[buf]);
+          return true;
+        };
+        for (int i = 0; i < min(2, n) && ok; ++i) ok = scores(i);
+        for (int i = 0; i < n && ok; ++i) {
+          const int s = i & 1, blk = dual ? i >> 1 : i;
+          ok = mbar_wait(&ctl.p_full[s], p_uses[s], abort_flag);
+          if (!ok) break;
+          ++p_uses[s];
+          const uint32_t p = pos + ring_v(dual, blk, nblk), st = p % kStages;
+          ok = mbar_wait(&ctl.kv_full[st], p / kStages, abort_flag);
+          if (!ok) break;
+          fence_async_smem();
+          tc_fence_after();
+          const uint64_t dv = operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes), kHalfBytes);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)                    // 16 keys each: two eight-row groups
+            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4),
+                   i >= 2 || k > 0);
+          if (!dual || s == 1) mma_commit(&ctl.kv_empty[st]);
+          if (i + 2 >= n) mma_commit(&ctl.o_full[s]);
+          if (i + 2 < n) ok = scores(i + 2);
+        }
+        pos += 2 * nblk;
+      }
+    }
+  } else {
+    // ---- softmax: this thread's row of its stream
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int s = warp >> 2, r = tid & 127;
+    const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + s * 128 + t_lane, t_o = tmem + 256 + s * 128 + t_lane;
+    const float scale = a.sm_scale * 1.4426950408889634f;
+    const float slack = 8.f / scale;                     // scores may exceed the kept maximum by this
+    char* const slots = static_cast<char*>(a.workspace) + 4096;
+    unsigned* const counters = static_cast<unsigned*>(a.workspace);
+    uint32_t s_uses = 0, o_uses = 0, j_uses = 0, pos = 0;
+    bool ok = true;
+    auto both_streams = [&]() {                          // barrier of the eight softmax warps, bounded
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.join);
+      const bool done = mbar_wait(&ctl.join, j_uses++, abort_flag);
+      return __all_sync(0xffffffffu, done) != 0;
+    };
+    for (int it = 0; ok; ++it) {
+      const int islot = it & (kItems - 1);
+      ok = mbar_wait(&ctl.item_full[islot], it / kItems, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      Item& o = ctl.items[islot];
+      if (!o.valid) break;
+      const int dual = o.dual, nblk = o.nblk, ntok = o.ntok;
+      const int t = (dual ? s * tile_tokens : 0) + r / G;
+      const bool live = r < tile_tokens * G && t < ntok;
+      const bool any_live = __any_sync(0xffffffffu, live);
+      const int p = o.pos0 + t;
+      // keys of this row; padding rows take all (they are computed and thrown away)
+      const int key_lo = live && a.window >= 0 ? static_cast<int>(max(0ll, static_cast<long long>(p) + 1 - a.window)) : 0;
+      const int key_hi = live ? p + 1 : INT_MAX;
+      const int first = o.k0 + o.blk0 * kBlk;
+      float m = -INFINITY, l = 0.f;
+      const int step = dual ? 1 : 2, blk_first = dual ? 0 : s;
+      for (int blk = blk_first; blk < nblk; blk += step) {
+        ok = mbar_wait(&ctl.s_full[s], s_uses, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++s_uses;
+        tc_fence_after();
+        const int kb = first + blk * kBlk;
+        if (any_live) {
+          uint32_t u[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, u[c]);
+          tmem_ld_wait();
+          const int c_lo = key_lo - kb, c_hi = key_hi > kb + kBlk ? kBlk : key_hi - kb;   // columns in [c_lo, c_hi)
+          if (__any_sync(0xffffffffu, c_lo > 0 || c_hi < kBlk)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i < c_lo || c * 32 + i >= c_hi) u[c][i] = 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[c][i]));
+          const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool grow = bm > m + slack || (m == -INFINITY && bm > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - bm) * scale);
+            if (grow) m = bm;
+            l *= f;
+            if (blk != blk_first) {                      // the product before this one has finished
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t w[32];
+                tmem_ld32(t_o + c * 32, w);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+                tmem_st32(t_o + c * 32, w);
+              }
+            }
+          }
+          const float ms = m == -INFINITY ? 0.f : m * scale;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e0 = ex2(fmaf(__uint_as_float(u[c][2 * i]), scale, -ms));
+              const float e1 = ex2(fmaf(__uint_as_float(u[c][2 * i + 1]), scale, -ms));
+              sum[i & 3] += e0 + e1;
+              w[i] = pack_bf16(e0, e1);
+            }
+            tmem_st16(t_s + c * 16, w);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        if (partly_attended(o, a.window, kb)) {
+          // A weight of zero does not silence an infinite or NaN value in the product.  Such values
+          // of a block that some rows attend only in part are taken out here and put back, for the
+          // rows that do attend them, when the unit ends.
+          const uint32_t vp = pos + ring_v(dual, blk, nblk), st = vp % kStages;
+          ok = mbar_wait(&ctl.kv_full[st], vp / kStages, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint32_t* v = reinterpret_cast<uint32_t*>(smem + kSmemKv + st * kTileBytes);
+          unsigned found = 0;
+#pragma unroll 4
+          for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(v + (i * 128 + r) * 4);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              found |= ((w[j] & 0x7f80u) == 0x7f80u || (w[j] & 0x7f800000u) == 0x7f800000u) ? 1u : 0u;
+          }
+          if (found) {
+            *reinterpret_cast<volatile unsigned*>(&o.nonfinite) = 1u;   // before any value is taken out
+            __threadfence_block();
+            for (int i = 0; i < kTileBytes / 16 / 128; ++i)
+              for (int j = 0; j < 4; ++j) {
+                uint32_t& w = v[(i * 128 + r) * 4 + j];
+                if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+                if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+              }
+          }
+          fence_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_full[s]);
+      }
+      if (!ok) break;
+      pos += 2 * nblk;
+      const bool worked = blk_first < nblk;
+      if (worked) {
+        ok = mbar_wait(&ctl.o_full[s], o_uses, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++o_uses;
+        tc_fence_after();
+      }
+      const bool join = o.parts > 1 || (!dual && nblk > 1);
+      __threadfence_block();
+      const bool refill = worked && *reinterpret_cast<volatile unsigned*>(&o.nonfinite) != 0u;
+      const int hq = o.kh * G + r % G;
+      const int64_t orow = static_cast<int64_t>(o.tok0 + t) * a.Hq + hq;
+      const bool direct = !join && live && (dual || s == 0);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float* part = reinterpret_cast<float*>(slots + static_cast<int64_t>(o.slot) * kSlotBytes);
+      if (any_live && (worked || direct)) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float v[32];
+          if (worked) {
+            uint32_t w[32];
+            tmem_ld32(t_o + c * 32, w);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          }
+          if (refill && live) {
+            for (int blk = blk_first; blk < nblk; blk += step) {
+              const int kb = first + blk * kBlk;
+              if (!partly_attended(o, a.window, kb)) continue;
+              for (int key = max(kb, key_lo); key < min(kb + kBlk, key_hi); ++key) {
+                const uint32_t* x = static_cast<const uint32_t*>(v_row(a, o, key));
+                if (x == nullptr) continue;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const uint32_t w = x[c * 16 + i];
+                  if ((w & 0x7f80u) == 0x7f80u) v[2 * i] += __uint_as_float(w << 16);
+                  if ((w & 0x7f800000u) == 0x7f800000u) v[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
+                }
+              }
+            }
+          }
+          if (direct) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + orow * 256 + c * 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = l == 0.f ? 0u : pack_bf16(v[i * 8 + 2 * j] * inv, v[i * 8 + 2 * j + 1] * inv);
+              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else if (live && join) {
+            float4* dst = reinterpret_cast<float4*>(part + (s * kRows + r) * 128 + c * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              __stcg(dst + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+          }
+        }
+      }
+      if (direct && a.lse)
+        a.lse[orow] = l == 0.f ? -INFINITY : (m * scale + log2f(l)) * 0.6931471805599453f;
+      if (join) {
+        if (live)
+          __stcg(reinterpret_cast<float2*>(part + kSlotFloats) + s * kRows + r, make_float2(m, l));
+        __threadfence();
+        ok = both_streams();
+        if (!ok) break;
+        if (tid == 0) {
+          ctl.last = o.parts == 1 || atomicInc(counters + o.cta0, o.parts - 1) == static_cast<unsigned>(o.parts - 1);
+          __threadfence();
+        }
+        ok = both_streams();
+        if (!ok) break;
+        if (ctl.last) {
+          // ---- join the parts of this unit: one warp a row, four dims a lane
+          const int rows = ntok * G;
+          const int per_part = dual ? 1 : 2;
+          for (int row = warp; row < rows; row += kSoftmaxWarps) {
+            const int token = row / G, g = row - token * G;
+            const int str = dual && token >= tile_tokens;
+            const int rr = str ? row - tile_tokens * G : row;
+            auto slot_of = [&](int i) {                  // contribution i: part i / per_part, stream
+              const int c = o.cta0 + i / per_part;
+              return slots + static_cast<int64_t>(2 * c + (c == o.cta0 ? 1 : 0)) * kSlotBytes;
+            };
+            auto lane_of = [&](int i) { return (dual ? str : i & 1) * kRows + rr; };
+            const int n = o.parts * per_part;
+            float mx = -INFINITY;
+            for (int i = lane; i < n; i += 32)
+              mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2*>(slot_of(i) + kSlotFloats * 4) + lane_of(i)).x);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float ms = mx == -INFINITY ? 0.f : mx * scale;
+            float lsum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+              const char* sl = slot_of(i);
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(sl + kSlotFloats * 4) + lane_of(i));
+              if (ml.y == 0.f) continue;                 // nothing attended in this part
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(sl) + lane_of(i) * 32 + lane);
+              const float f = ex2(ml.x * scale - ms);
+              lsum += ml.y * f;
+              acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
+            }
+            const float k = lsum == 0.f ? 0.f : 1.f / lsum;
+            const int64_t to = static_cast<int64_t>(o.tok0 + token) * a.Hq + o.kh * G + g;
+            uint2 w = make_uint2(0u, 0u);
+            if (lsum != 0.f) w = make_uint2(pack_bf16(acc.x * k, acc.y * k), pack_bf16(acc.z * k, acc.w * k));
+            *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + to * 256 + lane * 8) = w;
+            if (a.lse && lane == 0)
+              a.lse[to] = lsum == 0.f ? -INFINITY : (ms + log2f(lsum)) * 0.6931471805599453f;
+          }
+        }
+        ok = both_streams();                             // the slot and ctl.last are free again
+        if (!ok) break;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.item_empty[islot]);
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
 // One warp per (row, query head); a lane holds dims [4l, 4l+4).
 template <bool kE4m3>
-__global__ void __launch_bounds__(kWarps * 32) chunk_rows_kernel(const MacB200ChunkArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const MacB200ChunkArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
   if (task >= static_cast<int64_t>(a.q_rows) * a.Hq) return;
   const int row = static_cast<int>(task / a.Hq), hq = static_cast<int>(task - static_cast<int64_t>(row) * a.Hq);
   const int kh = hq / (a.Hq / a.Hkv);
@@ -89,7 +969,40 @@ __global__ void __launch_bounds__(kWarps * 32) chunk_rows_kernel(const MacB200Ch
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-int64_t workspace_bytes(int sms) { return static_cast<int64_t>(sms) * 16; }
+// counters (one a CTA), then two slots a CTA
+int64_t workspace_bytes(int sms) { return 4096 + 2 * static_cast<int64_t>(sms) * kSlotBytes; }
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                  CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled_fn() {
+  static EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(ptr);
+  }();
+  return fn;
+}
+
+// Sets the kernel up on the current device, once: its shared memory, and the check that it was
+// built with the registers that its warps trade among themselves (a build with fewer would wait
+// for them for ever).
+int prepare_kernel(int device) {
+  static std::atomic<int> ready[64];
+  if (device >= 0 && device < 64 && ready[device].load(std::memory_order_acquire)) return MAC_B200_OK;
+  cudaFuncAttributes attr{};
+  MAC_CUDA(cudaFuncGetAttributes(&attr, chunk_attention_kernel));
+  if (attr.numRegs * kThreads < 256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs)
+    return fail(MAC_B200_EUNSUPPORTED, "the chunk attention kernel was built with %d registers a thread",
+                attr.numRegs);
+  MAC_CUDA(cudaFuncSetAttribute(chunk_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  if (device >= 0 && device < 64) ready[device].store(1, std::memory_order_release);
+  return MAC_B200_OK;
+}
 
 int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
   MAC_REQUIRE(args != nullptr, "chunk args must not be null");
@@ -99,6 +1012,7 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
               "Hq must be Hkv times 1..16");
   MAC_REQUIRE(a.Hkv <= 1024, "Hkv must not exceed 1024");
   MAC_REQUIRE(a.B >= 0 && a.q_rows >= 0, "negative batch");
+  MAC_REQUIRE(a.B < (1 << 30) && a.q_rows < (1 << 30), "batch too large");
   MAC_REQUIRE(std::isfinite(a.sm_scale) && a.sm_scale > 0.f, "sm_scale must be positive");
   if (a.B == 0 || a.q_rows == 0) return MAC_B200_OK;
   MAC_REQUIRE(a.q && a.k && a.v && a.req_to_token && a.req_ids && a.offsets && a.kv_lens && a.out && a.workspace,
@@ -106,6 +1020,8 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
   MAC_REQUIRE(!e4m3 || (a.k_exp && a.v_exp), "the 8-bit pool needs its exponents");
   MAC_REQUIRE(a.kv_tokens > 0 && a.kv_tokens < (int64_t(1) << 31), "the pool must hold 1..2^31-1 rows");
   MAC_REQUIRE(a.req_to_token_rows > 0 && a.req_to_token_stride > 0, "req_to_token must not be empty");
+  MAC_REQUIRE(a.req_to_token_stride < (1 << 30), "req_to_token rows are too long");
+  MAC_REQUIRE(a.q_stride0 < (int64_t(1) << 38), "q row stride too large");
   MAC_REQUIRE(a.q_stride0 >= static_cast<int64_t>(a.Hq) * 128 && a.q_stride0 % 8 == 0,
               "q row stride must be a multiple of 8 and at least Hq*128");
   MAC_REQUIRE(on16(a.q) && on16(a.k) && on16(a.v) && on16(a.out) && on16(a.workspace),
@@ -116,12 +1032,27 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
   MAC_REQUIRE(a.workspace_bytes >= workspace_bytes(sms), "workspace holds %lld bytes, %lld are needed",
               static_cast<long long>(a.workspace_bytes), static_cast<long long>(workspace_bytes(sms)));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  const int64_t blocks = (static_cast<int64_t>(a.q_rows) * a.Hq + kWarps - 1) / kWarps;
-  MAC_REQUIRE(blocks < (int64_t(1) << 31), "chunk problem too large");
-  if (e4m3)
-    chunk_rows_kernel<true><<<static_cast<unsigned>(blocks), kWarps * 32, 0, stream>>>(a);
-  else
-    chunk_rows_kernel<false><<<static_cast<unsigned>(blocks), kWarps * 32, 0, stream>>>(a);
+  if (e4m3) {
+    const int64_t blocks = (static_cast<int64_t>(a.q_rows) * a.Hq + kRowWarps - 1) / kRowWarps;
+    MAC_REQUIRE(blocks < (int64_t(1) << 31), "chunk problem too large");
+    chunk_rows_kernel<true><<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, stream>>>(a);
+  } else {
+    MAC_REQUIRE(sms <= 1024, "too many multiprocessors");
+    if (const int rc = prepare_kernel(device)) return rc;
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (enc == nullptr) return fail(MAC_B200_EUNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+    alignas(64) CUtensorMap q_map;
+    const cuuint32_t ones[3] = {1u, 1u, 1u};
+    const int G = a.Hq / a.Hkv;
+    const cuuint64_t q_dims[3] = {128u, static_cast<cuuint64_t>(a.Hq), static_cast<cuuint64_t>(a.q_rows)};
+    const cuuint64_t q_strides[2] = {256u, static_cast<cuuint64_t>(a.q_stride0) * 2};
+    const cuuint32_t q_box[3] = {64u, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(kRows / G)};
+    const CUresult rc = enc(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), q_dims, q_strides, q_box,
+                      ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(MAC_B200_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
+    chunk_attention_kernel<<<sms, kThreads, kSmemBytes, stream>>>(a, q_map);
+  }
   MAC_CUDA(cudaGetLastError());
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   return MAC_B200_OK;
