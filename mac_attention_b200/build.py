@@ -69,7 +69,8 @@ def shim_is_stale() -> bool:
     if not SHIM.exists():
         return True
     t = SHIM.stat().st_mtime
-    return any(d.stat().st_mtime > t for d in (SHIM_SRC, PKG.parent / "include" / "mac_b200.h"))
+    include = PKG.parent / "include"
+    return any(d.stat().st_mtime > t for d in (SHIM_SRC, include / "mac_b200.h", include / "mac_b200_chunk.h"))
 
 
 def build_shim(force: bool = False, verbose: bool = False) -> Path:

@@ -1,4 +1,4 @@
-// Torch-extension shim of the decode operator: the pybind module the reference
+// Torch-extension shim of the per-step operators.  The decode operator: the pybind module the reference
 // ships for mac_persistent_decode_bf16 (mac_decode_persistent.cu:4962-5030 and
 // 5526-5529 in the reference project), re-expressed over the C ABI.
 //
@@ -10,6 +10,10 @@
 // exceptions: kShimCheckFailed with the text at last_error() for a failed
 // check (the Python operator raises the RuntimeError the reference's
 // TORCH_CHECK would), else the C ABI's own status code.
+//
+// The chunk attention and the 8-bit pool's operators (mac_b200_chunk.h; not in the reference) go
+// the same way below it: a step of a served model calls them once a layer, and through ctypes a
+// call cost 20-35 us of host time.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -19,6 +23,7 @@
 #include <string>
 
 #include "../../include/mac_b200.h"
+#include "../../include/mac_b200_chunk.h"
 
 namespace {
 
@@ -358,6 +363,250 @@ int decode(
                                  : mac_b200_persistent_decode_bf16(&a, stream);
 }
 
+// ---- chunk attention and the 8-bit pool ------------------------------------------------------
+int check_on(const Tensor& t, const char* name, const at::Device& device) {
+  REQUIRE(t.is_cuda(), name, " must be CUDA");
+  REQUIRE(t.device() == device, name, " must be on ", device.str());
+  return 0;
+}
+
+int check_row_pool(const Tensor& k, const char* k_name, const Tensor& v, const char* v_name,
+                   at::ScalarType dtype, const at::Device& device) {
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = i ? v : k;
+    const char* name = i ? v_name : k_name;
+    REQUIRE_OK(check_on(t, name, device));
+    REQUIRE(t.scalar_type() == dtype, name, " has wrong dtype");
+    REQUIRE(t.dim() == 3 && t.size(2) == 128, name, " must be [T,Hkv,128]");
+    REQUIRE(t.is_contiguous(), name, " must be contiguous");
+  }
+  REQUIRE(v.sizes() == k.sizes(), v_name, " must match ", k_name);
+  REQUIRE(k.size(1) > 0, k_name, " must be [T,Hkv,128]");
+  return 0;
+}
+
+int check_exponents(const Tensor& pool, const Tensor& k_exp, const Tensor& v_exp) {
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = i ? v_exp : k_exp;
+    const char* name = i ? "v_exp" : "k_exp";
+    REQUIRE_OK(check_on(t, name, pool.device()));
+    REQUIRE(t.scalar_type() == at::kByte, name, " has wrong dtype");
+    REQUIRE(t.dim() == 2 && t.size(0) == pool.size(0) && t.size(1) == pool.size(1), name, " must be [T,Hkv]");
+    REQUIRE(t.is_contiguous(), name, " must be contiguous");
+  }
+  return 0;
+}
+
+int check_locs(const Tensor& t, const char* name, int64_t rows, const at::Device& device) {
+  REQUIRE_OK(check_on(t, name, device));
+  REQUIRE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+  REQUIRE(t.dim() == 1 && t.is_contiguous(), name, " must be contiguous with rank 1");
+  REQUIRE(t.size(0) >= rows, name, " is shorter than the batch");
+  return 0;
+}
+
+void* stream_of(const at::Device& device) {
+  return static_cast<void*>(c10::cuda::getCurrentCUDAStream(device.index()).stream());
+}
+
+// A null k_exp means the bf16 pool.  window < 0: none.
+int chunk_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& k_exp,
+                    const OptTensor& v_exp, const Tensor& req_to_token, const Tensor& req_ids,
+                    const Tensor& offsets, const Tensor& kv_lens, const Tensor& out, const OptTensor& lse,
+                    const Tensor& workspace, double sm_scale, int64_t window) {
+  const bool e4m3 = k_exp.has_value();
+  REQUIRE(q.is_cuda(), "q must be CUDA");
+  const at::Device device = q.device();
+  if (e4m3) {
+    REQUIRE_OK(check_row_pool(k, "k_pool", v, "v_pool", at::kFloat8_e4m3fn, device));
+    REQUIRE_OK(check_exponents(k, *k_exp, *v_exp));
+  } else {
+    REQUIRE_OK(check_row_pool(k, "k_buffer", v, "v_buffer", at::kBFloat16, device));
+  }
+  REQUIRE(q.scalar_type() == at::kBFloat16, "q has wrong dtype");
+  REQUIRE(q.dim() == 3 && q.size(2) == 128, "q must be [rows,Hq,128]");
+  const int64_t rows = q.size(0), Hq = q.size(1);
+  REQUIRE(Hq > 0 && q.stride(2) == 1 && (Hq == 1 || q.stride(1) == 128), "q rows must be contiguous");
+  REQUIRE_OK(check_on(out, "out", device));
+  REQUIRE(out.scalar_type() == at::kBFloat16, "out has wrong dtype");
+  REQUIRE(out.sizes() == q.sizes() && out.is_contiguous(), "out must be contiguous and match q");
+  if (lse.has_value()) {
+    REQUIRE_OK(check_on(*lse, "lse", device));
+    REQUIRE(lse->scalar_type() == at::kFloat, "lse has wrong dtype");
+    REQUIRE(lse->dim() == 2 && lse->size(0) == rows && lse->size(1) == Hq && lse->is_contiguous(),
+            "lse must be [rows,Hq]");
+  }
+  const int64_t Hkv = k.size(1);
+  REQUIRE(Hq % Hkv == 0, "Hq must be divisible by Hkv");
+  REQUIRE_OK(check_on(req_to_token, "req_to_token", device));
+  REQUIRE(req_to_token.scalar_type() == at::kInt && req_to_token.dim() == 2 && req_to_token.is_contiguous(),
+          "req_to_token must be contiguous int32 [rows,cols]");
+  const Tensor* lists[3] = {&req_ids, &offsets, &kv_lens};
+  const char* names[3] = {"req_ids", "offsets", "kv_lens"};
+  for (int i = 0; i < 3; ++i) {
+    REQUIRE_OK(check_on(*lists[i], names[i], device));
+    REQUIRE(lists[i]->scalar_type() == at::kInt && lists[i]->dim() == 1 && lists[i]->is_contiguous(), names[i],
+            " must be contiguous int32 [B]");
+  }
+  const int64_t B = req_ids.size(0);
+  REQUIRE(offsets.size(0) == B + 1, "offsets must be [B+1]");
+  REQUIRE(kv_lens.size(0) == B, "kv_lens must be [B]");
+  REQUIRE_OK(check_on(workspace, "workspace", device));
+  REQUIRE(workspace.is_contiguous(), "workspace must be contiguous");
+  REQUIRE(rows < (1ll << 30) && B < (1ll << 30) && Hq < (1ll << 30) && req_to_token.size(0) < (1ll << 30) &&
+              req_to_token.size(1) < (1ll << 30),
+          "batch too large");
+  if (rows == 0 || B == 0) return 0;
+  MacB200ChunkArgs a{};
+  a.B = static_cast<int32_t>(B);
+  a.Hq = static_cast<int32_t>(Hq);
+  a.Hkv = static_cast<int32_t>(Hkv);
+  a.D = 128;
+  a.q_rows = static_cast<int32_t>(rows);
+  a.req_to_token_rows = static_cast<int32_t>(req_to_token.size(0));
+  a.req_to_token_stride = static_cast<int32_t>(req_to_token.size(1));
+  a.window = static_cast<int32_t>(window < 0 ? -1 : window < 0x7fffffff ? window : 0x7fffffff);
+  a.kv_tokens = k.size(0);
+  a.q_stride0 = rows > 1 ? q.stride(0) : Hq * 128;
+  a.workspace_bytes = static_cast<int64_t>(workspace.nbytes());
+  a.sm_scale = static_cast<float>(sm_scale);
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_exp = e4m3 ? k_exp->data_ptr<uint8_t>() : nullptr;
+  a.v_exp = e4m3 ? v_exp->data_ptr<uint8_t>() : nullptr;
+  a.req_to_token = req_to_token.data_ptr<int32_t>();
+  a.req_ids = req_ids.data_ptr<int32_t>();
+  a.offsets = offsets.data_ptr<int32_t>();
+  a.kv_lens = kv_lens.data_ptr<int32_t>();
+  a.out = out.data_ptr();
+  a.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
+  a.workspace = workspace.data_ptr();
+  const c10::cuda::CUDAGuard guard(device);
+  return e4m3 ? mac_b200_chunk_attention_e4m3(&a, stream_of(device))
+              : mac_b200_chunk_attention_bf16(&a, stream_of(device));
+}
+
+int quantize_args(MacB200QuantizeKvArgs& a, const Tensor& k, const Tensor& v, const Tensor& k_pool,
+                  const Tensor& v_pool, const Tensor& k_exp, const Tensor& v_exp, const Tensor& cache_locs) {
+  REQUIRE(k.is_cuda(), "k must be CUDA");
+  const at::Device device = k.device();
+  REQUIRE_OK(check_on(v, "v", device));
+  REQUIRE_OK(check_row_pool(k_pool, "k_pool", v_pool, "v_pool", at::kFloat8_e4m3fn, device));
+  REQUIRE_OK(check_exponents(k_pool, k_exp, v_exp));
+  const int64_t Hkv = k_pool.size(1);
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = i ? v : k;
+    const char* name = i ? "v" : "k";
+    REQUIRE(t.scalar_type() == at::kBFloat16, name, " has wrong dtype");
+    REQUIRE(t.dim() == 2 && t.size(1) == Hkv * 128, name, " must be [N,Hkv*128]");
+    REQUIRE(t.stride(1) == 1, name, " must have contiguous last dimension");
+  }
+  REQUIRE(v.size(0) == k.size(0), "k/v batch mismatch");
+  REQUIRE_OK(check_locs(cache_locs, "cache_locs", k.size(0), device));
+  a.N = k.size(0);
+  a.Hkv = static_cast<int32_t>(Hkv);
+  a.D = 128;
+  a.cache_locs_i64 = cache_locs.scalar_type() == at::kLong ? 1 : 0;
+  a.k_stride0 = k.stride(0);
+  a.v_stride0 = v.stride(0);
+  a.kv_pool_tokens = k_pool.size(0);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_pool = k_pool.data_ptr();
+  a.v_pool = v_pool.data_ptr();
+  a.k_exp = k_exp.data_ptr<uint8_t>();
+  a.v_exp = v_exp.data_ptr<uint8_t>();
+  a.cache_locs = cache_locs.data_ptr();
+  return 0;
+}
+
+int quantize_kv(const Tensor& k, const Tensor& v, const Tensor& k_pool, const Tensor& v_pool,
+                const Tensor& k_exp, const Tensor& v_exp, const Tensor& cache_locs) {
+  MacB200QuantizeKvArgs a{};
+  REQUIRE_OK(quantize_args(a, k, v, k_pool, v_pool, k_exp, v_exp, cache_locs));
+  if (a.N == 0) return 0;
+  const c10::cuda::CUDAGuard guard(k.device());
+  return mac_b200_quantize_kv_e4m3(&a, stream_of(k.device()));
+}
+
+int rope_quantize_kv(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_post,
+                     const Tensor& k_pool, const Tensor& v_pool, const Tensor& k_exp, const Tensor& v_exp,
+                     const Tensor& cos_sin_cache, const Tensor& positions, const Tensor& cache_locs,
+                     int64_t head_dim, bool is_neox) {
+  REQUIRE(head_dim == 128, "the 8-bit pool needs head_dim 128");
+  MacB200QuantizeKvArgs a{};
+  REQUIRE_OK(quantize_args(a, k, v, k_pool, v_pool, k_exp, v_exp, cache_locs));
+  const at::Device device = k.device();
+  REQUIRE_OK(check_on(q, "q", device));
+  REQUIRE_OK(check_on(q_post, "q_post", device));
+  REQUIRE_OK(check_on(cos_sin_cache, "cos_sin_cache", device));
+  REQUIRE(q.scalar_type() == at::kBFloat16, "q has wrong dtype");
+  REQUIRE(q.dim() == 2 && q.size(0) == a.N && q.size(1) > 0 && q.size(1) % 128 == 0, "q must be [N,Hq*128]");
+  REQUIRE(q.stride(1) == 1, "q must have contiguous last dimension");
+  const int64_t Hq = q.size(1) / 128;
+  REQUIRE(q_post.scalar_type() == at::kBFloat16, "q_post has wrong dtype");
+  REQUIRE(q_post.dim() == 3 && q_post.size(0) >= a.N && q_post.size(1) == Hq && q_post.size(2) == 128,
+          "q_post must be [>=N,Hq,128]");
+  REQUIRE(q_post.is_contiguous(), "q_post must be contiguous");
+  REQUIRE(cos_sin_cache.scalar_type() == at::kFloat, "cos_sin_cache has wrong dtype");
+  REQUIRE(cos_sin_cache.dim() == 2 && cos_sin_cache.stride(1) == 1,
+          "cos_sin_cache must have contiguous last dimension");
+  REQUIRE_OK(check_locs(positions, "positions", a.N, device));
+  const int64_t rotary_dim = cos_sin_cache.size(1);
+  REQUIRE(rotary_dim > 0 && rotary_dim <= 128 && rotary_dim % 2 == 0, "invalid rotary_dim");
+  if (a.N == 0) return 0;
+  a.Hq = static_cast<int32_t>(Hq);
+  a.rotary_dim = static_cast<int32_t>(rotary_dim);
+  a.is_neox = is_neox ? 1 : 0;
+  a.positions_i64 = positions.scalar_type() == at::kLong ? 1 : 0;
+  a.q_stride0 = q.stride(0);
+  a.cos_sin_stride0 = cos_sin_cache.stride(0);
+  a.max_positions = cos_sin_cache.size(0);
+  a.q = q.data_ptr();
+  a.q_post = q_post.data_ptr();
+  a.cos_sin_cache = cos_sin_cache.data_ptr<float>();
+  a.positions = positions.data_ptr();
+  const c10::cuda::CUDAGuard guard(device);
+  return mac_b200_quantize_kv_e4m3(&a, stream_of(device));
+}
+
+int dequantize_kv(const Tensor& k_pool, const Tensor& v_pool, const Tensor& k_exp, const Tensor& v_exp,
+                  const Tensor& src_locs, const Tensor& k_buffer, const Tensor& v_buffer,
+                  const OptTensor& dst_locs) {
+  REQUIRE(k_pool.is_cuda(), "k_pool must be CUDA");
+  const at::Device device = k_pool.device();
+  REQUIRE_OK(check_row_pool(k_pool, "k_pool", v_pool, "v_pool", at::kFloat8_e4m3fn, device));
+  REQUIRE_OK(check_exponents(k_pool, k_exp, v_exp));
+  REQUIRE_OK(check_row_pool(k_buffer, "k_buffer", v_buffer, "v_buffer", at::kBFloat16, device));
+  REQUIRE(k_buffer.size(1) == k_pool.size(1), "k_buffer must have the pool's heads");
+  REQUIRE_OK(check_locs(src_locs, "src_locs", 0, device));
+  MacB200DequantizeKvArgs a{};
+  a.N = src_locs.size(0);
+  if (dst_locs.has_value()) {
+    REQUIRE_OK(check_locs(*dst_locs, "dst_locs", a.N, device));
+    a.dst_locs = dst_locs->data_ptr();
+    a.dst_locs_i64 = dst_locs->scalar_type() == at::kLong ? 1 : 0;
+  } else {
+    REQUIRE(k_buffer.size(0) >= a.N, "k_buffer is shorter than src_locs");
+  }
+  if (a.N == 0) return 0;
+  a.Hkv = static_cast<int32_t>(k_pool.size(1));
+  a.D = 128;
+  a.src_locs_i64 = src_locs.scalar_type() == at::kLong ? 1 : 0;
+  a.src_tokens = k_pool.size(0);
+  a.dst_tokens = k_buffer.size(0);
+  a.k_pool = k_pool.data_ptr();
+  a.v_pool = v_pool.data_ptr();
+  a.k_exp = k_exp.data_ptr<uint8_t>();
+  a.v_exp = v_exp.data_ptr<uint8_t>();
+  a.src_locs = src_locs.data_ptr();
+  a.k_buffer = k_buffer.data_ptr();
+  a.v_buffer = v_buffer.data_ptr();
+  const c10::cuda::CUDAGuard guard(device);
+  return mac_b200_dequantize_kv_e4m3(&a, stream_of(device));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -369,4 +618,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "entry (0: allocating, 1: fixed scratch block) followed by the reference operator's 68 "
         "positional arguments; task lists and partial buffers may be None (lean call); returns "
         "the C ABI's status code");
+  m.def("chunk_attention", &chunk_attention,
+        "chunk attention over the bf16 pool (no exponents) or the e4m3 pool; returns the C ABI's status code");
+  m.def("quantize_kv", &quantize_kv, "rows of k and v into the e4m3 pool; returns the C ABI's status code");
+  m.def("rope_quantize_kv", &rope_quantize_kv,
+        "the same behind the decode rotation; returns the C ABI's status code");
+  m.def("dequantize_kv", &dequantize_kv,
+        "rows of the e4m3 pool into a bf16 pool; returns the C ABI's status code");
 }

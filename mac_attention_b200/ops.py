@@ -8,6 +8,8 @@ what the reference launcher checks (same messages, ``RuntimeError``), fills the
 plain-C argument struct and calls the C ABI on torch's current stream.  The
 decode operators -- the per-step hot call -- do that in a compiled
 torch-extension shim (``csrc/mac_b200_torch.cpp``), the others through ctypes.
+The chunk attention and the operators of the 8-bit K/V pool (not in the
+reference; ``include/mac_b200_chunk.h``) go through the shim too.
 """
 from __future__ import annotations
 
@@ -426,82 +428,12 @@ def mac_update_then_downdate_bf16_inplace(out1, lse1, out2, lse2) -> None:
             _stream_ptr(out1.device)))
 
 
-_E4M3, _U8 = torch.float8_e4m3fn, torch.uint8
-
-
-def _check_on(device, **tensors) -> None:
-    """The tensors of one call are CUDA tensors of one device."""
-    for name, t in tensors.items():
-        _req(t.is_cuda, f"{name} must be CUDA")
-        _req(t.device == device, f"{name} must be on {device}")
-
-
-def _check_row_pool(k, v, dtype, names) -> None:
-    for name, t in zip(names, (k, v)):
-        _req(t.dtype == dtype, f"{name} has wrong dtype")
-        _req(t.dim() == 3 and t.shape[2] == 128, f"{name} must be [T,Hkv,128]")
-        _req(t.is_contiguous(), f"{name} must be contiguous")
-    _req(v.shape == k.shape, f"{names[1]} must match {names[0]}")
-
-
-def _check_exponents(k_pool, k_exp, v_exp) -> None:
-    for name, t in (("k_exp", k_exp), ("v_exp", v_exp)):
-        _req(t.dtype == _U8, f"{name} has wrong dtype")
-        _req(tuple(t.shape) == tuple(k_pool.shape[:2]), f"{name} must be [T,Hkv]")
-        _req(t.is_contiguous(), f"{name} must be contiguous")
-
-
-def _check_locs(name, t, rows) -> None:
-    _req(t.dtype in (_I32, _I64), f"{name} must be int32 or int64")
-    _req(t.dim() == 1 and t.is_contiguous(), f"{name} must be contiguous with rank 1")
-    _req(t.shape[0] >= rows, f"{name} is shorter than the batch")
-
-
-def _chunk_attention(entry, q, k, v, k_exp, v_exp, req_to_token, req_ids, offsets, kv_lens, out, lse,
-                     workspace, sm_scale, window) -> None:
-    lib = _abi.load_library()
-    _check_on(q.device, q=q, k=k, v=v, req_to_token=req_to_token, req_ids=req_ids, offsets=offsets,
-              kv_lens=kv_lens, out=out, workspace=workspace)
-    _req(q.dtype == _BF16, "q has wrong dtype")
-    _req(q.dim() == 3 and q.shape[2] == 128, "q must be [rows,Hq,128]")
-    rows, Hq = q.shape[0], q.shape[1]
-    _req(Hq > 0 and q.stride(2) == 1 and (Hq == 1 or q.stride(1) == 128), "q rows must be contiguous")
-    _req(out.dtype == _BF16, "out has wrong dtype")
-    _req(out.shape == q.shape and out.is_contiguous(), "out must be contiguous and match q")
-    if lse is not None:
-        _check_on(q.device, lse=lse)
-        _req(lse.dtype == _F32, "lse has wrong dtype")
-        _req(tuple(lse.shape) == (rows, Hq) and lse.is_contiguous(), "lse must be [rows,Hq]")
-    Hkv = k.shape[1]
-    _req(Hkv > 0 and Hq % Hkv == 0, "Hq must be divisible by Hkv")
-    _req(req_to_token.dtype == _I32 and req_to_token.dim() == 2 and req_to_token.is_contiguous(),
-         "req_to_token must be contiguous int32 [rows,cols]")
-    for name, t in (("req_ids", req_ids), ("offsets", offsets), ("kv_lens", kv_lens)):
-        _req(t.dtype == _I32 and t.dim() == 1 and t.is_contiguous(), f"{name} must be contiguous int32 [B]")
-    B = req_ids.shape[0]
-    _req(offsets.shape[0] == B + 1, "offsets must be [B+1]")
-    _req(kv_lens.shape[0] == B, "kv_lens must be [B]")
-    _req(workspace.is_contiguous(), "workspace must be contiguous")
-    _req(window is None or int(window) >= 0, "negative window")
-    if rows == 0 or B == 0:
-        return
-    a = _abi.MacB200ChunkArgs()
-    a.B, a.Hq, a.Hkv, a.D, a.q_rows = B, Hq, Hkv, 128, rows
-    a.req_to_token_rows, a.req_to_token_stride = req_to_token.shape
-    a.window = -1 if window is None else min(int(window), 2**31 - 1)
-    a.kv_tokens = k.shape[0]
-    a.q_stride0 = q.stride(0) if rows > 1 else Hq * 128
-    a.workspace_bytes = workspace.numel() * workspace.element_size()
-    a.sm_scale = float(128 ** -0.5 if sm_scale is None else sm_scale)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.k_exp = None if k_exp is None else k_exp.data_ptr()
-    a.v_exp = None if v_exp is None else v_exp.data_ptr()
-    a.req_to_token, a.req_ids = req_to_token.data_ptr(), req_ids.data_ptr()
-    a.offsets, a.kv_lens = offsets.data_ptr(), kv_lens.data_ptr()
-    a.out, a.lse = out.data_ptr(), None if lse is None else lse.data_ptr()
-    a.workspace = workspace.data_ptr()
-    with torch.cuda.device(q.device):
-        _abi.check(getattr(lib, entry)(C.byref(a), _stream_ptr(q.device)))
+def _scale_and_window(sm_scale, window):
+    """(scale, window) as the shim takes them: 1/sqrt(128) by default, -1 for no window."""
+    if window is not None:
+        window = int(window)
+        _req(window >= 0, "negative window")
+    return float(128 ** -0.5 if sm_scale is None else sm_scale), -1 if window is None else min(window, 2**31 - 1)
 
 
 def mac_chunk_attention_bf16(q, k_buffer, v_buffer, req_to_token, req_ids, offsets, kv_lens, out, lse,
@@ -523,9 +455,9 @@ def mac_chunk_attention_bf16(q, k_buffer, v_buffer, req_to_token, req_ids, offse
     ``workspace`` is from :func:`mac_attention_b200.make_chunk_attention_workspace`; calls that
     may overlap on the device need one each.  Entries that lie outside their tables are
     reported by :func:`query_status` (``include/mac_b200_chunk.h`` says what they give)."""
-    _check_row_pool(k_buffer, v_buffer, _BF16, ("k_buffer", "v_buffer"))
-    _chunk_attention("mac_b200_chunk_attention_bf16", q, k_buffer, v_buffer, None, None, req_to_token,
-                     req_ids, offsets, kv_lens, out, lse, workspace, sm_scale, window)
+    _raise_on_failure(_load_shim().chunk_attention(
+        q, k_buffer, v_buffer, None, None, req_to_token, req_ids, offsets, kv_lens, out, lse, workspace,
+        *_scale_and_window(sm_scale, window)))
 
 
 def mac_chunk_attention_e4m3(q, k_pool, v_pool, k_exp, v_exp, req_to_token, req_ids, offsets, kv_lens,
@@ -533,37 +465,11 @@ def mac_chunk_attention_e4m3(q, k_pool, v_pool, k_exp, v_exp, req_to_token, req_
     """:func:`mac_chunk_attention_bf16` over an 8-bit pool: codes ``[T,Hkv,128]`` e4m3 and one
     exponent byte per row ``[T,Hkv]`` (``include/mac_b200_chunk.h`` has the format).  The result
     is that of the bf16 operator on the rows that :func:`mac_dequantize_kv_e4m3` reads back."""
-    _check_row_pool(k_pool, v_pool, _E4M3, ("k_pool", "v_pool"))
-    _check_exponents(k_pool, k_exp, v_exp)
-    _check_on(q.device, k_exp=k_exp, v_exp=v_exp)
-    _chunk_attention("mac_b200_chunk_attention_e4m3", q, k_pool, v_pool, k_exp, v_exp, req_to_token,
-                     req_ids, offsets, kv_lens, out, lse, workspace, sm_scale, window)
-
-
-def _quantize_args(k, v, k_pool, v_pool, k_exp, v_exp, cache_locs):
-    _check_on(k.device, k=k, v=v, k_pool=k_pool, v_pool=v_pool, k_exp=k_exp, v_exp=v_exp,
-              cache_locs=cache_locs)
-    _check_row_pool(k_pool, v_pool, _E4M3, ("k_pool", "v_pool"))
-    _check_exponents(k_pool, k_exp, v_exp)
-    Hkv = k_pool.shape[1]
-    _req(Hkv > 0, "k_pool must be [T,Hkv,128]")
-    for name, t in (("k", k), ("v", v)):
-        _req(t.dtype == _BF16, f"{name} has wrong dtype")
-        _req(t.dim() == 2 and t.shape[1] == Hkv * 128, f"{name} must be [N,Hkv*128]")
-        _req(t.stride(1) == 1, f"{name} must have contiguous last dimension")
-    N = k.shape[0]
-    _req(v.shape[0] == N, "k/v batch mismatch")
-    _check_locs("cache_locs", cache_locs, N)
-    a = _abi.MacB200QuantizeKvArgs()
-    a.N, a.Hkv, a.D = N, Hkv, 128
-    a.cache_locs_i64 = 1 if cache_locs.dtype == _I64 else 0
-    a.k_stride0, a.v_stride0 = k.stride(0), v.stride(0)
-    a.kv_pool_tokens = k_pool.shape[0]
-    a.k, a.v = k.data_ptr(), v.data_ptr()
-    a.k_pool, a.v_pool = k_pool.data_ptr(), v_pool.data_ptr()
-    a.k_exp, a.v_exp = k_exp.data_ptr(), v_exp.data_ptr()
-    a.cache_locs = cache_locs.data_ptr()
-    return a
+    if k_exp is None or v_exp is None:
+        raise TypeError("k_exp and v_exp must be tensors")
+    _raise_on_failure(_load_shim().chunk_attention(
+        q, k_pool, v_pool, k_exp, v_exp, req_to_token, req_ids, offsets, kv_lens, out, lse, workspace,
+        *_scale_and_window(sm_scale, window)))
 
 
 def mac_quantize_kv_e4m3(k, v, k_pool, v_pool, k_exp, v_exp, cache_locs) -> None:
@@ -572,12 +478,7 @@ def mac_quantize_kv_e4m3(k, v, k_pool, v_pool, k_exp, v_exp, cache_locs) -> None
     scale per row as its exponent byte into ``k_exp`` / ``v_exp`` ``[T,Hkv]``
     (``include/mac_b200_chunk.h`` has the format).  Entries of ``cache_locs`` outside the pool
     are skipped (padding); those inside have to be distinct."""
-    lib = _abi.load_library()
-    a = _quantize_args(k, v, k_pool, v_pool, k_exp, v_exp, cache_locs)
-    if a.N == 0:
-        return
-    with torch.cuda.device(k.device):
-        _abi.check(lib.mac_b200_quantize_kv_e4m3(C.byref(a), _stream_ptr(k.device)))
+    _raise_on_failure(_load_shim().quantize_kv(k, v, k_pool, v_pool, k_exp, v_exp, cache_locs))
 
 
 def mac_decode_rope_quantize_kv_e4m3(q, k, v, q_post, k_pool, v_pool, k_exp, v_exp, cos_sin_cache,
@@ -589,36 +490,8 @@ def mac_decode_rope_quantize_kv_e4m3(q, k, v, q_post, k_pool, v_pool, k_exp, v_e
     difference that ``q``, ``k``, ``v`` stay as they are: ``q`` itself is the pre-RoPE query.
     A token whose position lies outside ``cos_sin_cache`` is skipped and reported by
     :func:`query_status`."""
-    lib = _abi.load_library()
-    _req(int(head_dim) == 128, "the 8-bit pool needs head_dim 128")
-    _check_on(k.device, q=q, q_post=q_post, cos_sin_cache=cos_sin_cache, positions=positions)
-    a = _quantize_args(k, v, k_pool, v_pool, k_exp, v_exp, cache_locs)
-    N = a.N
-    _req(q.dtype == _BF16, "q has wrong dtype")
-    _req(q.dim() == 2 and q.shape[0] == N and q.shape[1] > 0 and q.shape[1] % 128 == 0,
-         "q must be [N,Hq*128]")
-    _req(q.stride(1) == 1, "q must have contiguous last dimension")
-    Hq = q.shape[1] // 128
-    _req(q_post.dtype == _BF16, "q_post has wrong dtype")
-    _req(q_post.dim() == 3 and q_post.shape[0] >= N and tuple(q_post.shape[1:]) == (Hq, 128),
-         "q_post must be [>=N,Hq,128]")
-    _req(q_post.is_contiguous(), "q_post must be contiguous")
-    _req(cos_sin_cache.dtype == _F32, "cos_sin_cache has wrong dtype")
-    _req(cos_sin_cache.dim() == 2 and cos_sin_cache.stride(1) == 1,
-         "cos_sin_cache must have contiguous last dimension")
-    _check_locs("positions", positions, N)
-    rotary_dim = cos_sin_cache.shape[1]
-    _req(0 < rotary_dim <= 128 and rotary_dim % 2 == 0, "invalid rotary_dim")
-    if N == 0:
-        return
-    a.Hq, a.rotary_dim, a.is_neox = Hq, rotary_dim, 1 if is_neox else 0
-    a.positions_i64 = 1 if positions.dtype == _I64 else 0
-    a.q_stride0, a.cos_sin_stride0 = q.stride(0), cos_sin_cache.stride(0)
-    a.max_positions = cos_sin_cache.shape[0]
-    a.q, a.q_post = q.data_ptr(), q_post.data_ptr()
-    a.cos_sin_cache, a.positions = cos_sin_cache.data_ptr(), positions.data_ptr()
-    with torch.cuda.device(k.device):
-        _abi.check(lib.mac_b200_quantize_kv_e4m3(C.byref(a), _stream_ptr(k.device)))
+    _raise_on_failure(_load_shim().rope_quantize_kv(q, k, v, q_post, k_pool, v_pool, k_exp, v_exp, cos_sin_cache,
+                                                    positions, cache_locs, int(head_dim), bool(is_neox)))
 
 
 def mac_dequantize_kv_e4m3(k_pool, v_pool, k_exp, v_exp, src_locs, k_buffer, v_buffer,
@@ -628,35 +501,8 @@ def mac_dequantize_kv_e4m3(k_pool, v_pool, k_exp, v_exp, src_locs, k_buffer, v_b
     the values it stands for.  Brings a parked request back for operators that read the bf16
     pool, the MAC decode step among them.  Entries outside their pool are skipped (padding);
     destinations inside have to be distinct."""
-    lib = _abi.load_library()
-    _check_on(k_pool.device, k_pool=k_pool, v_pool=v_pool, k_exp=k_exp, v_exp=v_exp, src_locs=src_locs,
-              k_buffer=k_buffer, v_buffer=v_buffer)
-    _check_row_pool(k_pool, v_pool, _E4M3, ("k_pool", "v_pool"))
-    _check_exponents(k_pool, k_exp, v_exp)
-    _check_row_pool(k_buffer, v_buffer, _BF16, ("k_buffer", "v_buffer"))
-    Hkv = k_pool.shape[1]
-    _req(Hkv > 0 and k_buffer.shape[1] == Hkv, "k_buffer must have the pool's heads")
-    _check_locs("src_locs", src_locs, 0)
-    N = src_locs.shape[0]
-    if dst_locs is not None:
-        _check_on(k_pool.device, dst_locs=dst_locs)
-        _check_locs("dst_locs", dst_locs, N)
-    else:
-        _req(k_buffer.shape[0] >= N, "k_buffer is shorter than src_locs")
-    if N == 0:
-        return
-    a = _abi.MacB200DequantizeKvArgs()
-    a.N, a.Hkv, a.D = N, Hkv, 128
-    a.src_locs_i64 = 1 if src_locs.dtype == _I64 else 0
-    a.src_tokens, a.dst_tokens = k_pool.shape[0], k_buffer.shape[0]
-    a.k_pool, a.v_pool = k_pool.data_ptr(), v_pool.data_ptr()
-    a.k_exp, a.v_exp = k_exp.data_ptr(), v_exp.data_ptr()
-    a.src_locs = src_locs.data_ptr()
-    a.k_buffer, a.v_buffer = k_buffer.data_ptr(), v_buffer.data_ptr()
-    if dst_locs is not None:
-        a.dst_locs, a.dst_locs_i64 = dst_locs.data_ptr(), 1 if dst_locs.dtype == _I64 else 0
-    with torch.cuda.device(k_pool.device):
-        _abi.check(lib.mac_b200_dequantize_kv_e4m3(C.byref(a), _stream_ptr(k_pool.device)))
+    _raise_on_failure(_load_shim().dequantize_kv(k_pool, v_pool, k_exp, v_exp, src_locs, k_buffer, v_buffer,
+                                                 dst_locs))
 
 
 def query_status(device=None) -> int:
