@@ -3,18 +3,19 @@
 //
 // Rows.  A KV head's G query heads see the same keys, so the rows of a tile are (token, query
 // head) pairs: 128/G tokens x G heads fill the 128 rows of a tcgen05 product.  A UNIT of work is
-// (request, KV head, up to two tiles of rows) with the keys that its rows attend together, in
+// (request, KV head, one or two tiles of rows) with the keys that its rows attend together, in
 // blocks of 128 keys.  Two tiles ("dual") share every staged K/V block, which halves the traffic
-// through shared memory; a unit whose rows fit one tile ("single": decode, drafted tokens, a
-// prompt's remainder) lets its two softmax streams take alternate blocks of the same rows and
-// joins the two results at the end.  Either way two streams are in flight, and while one is in its
-// softmax the other's products run.
+// through shared memory; in a unit of one tile ("single": decode, drafted tokens, a prompt's
+// remainder, and every unit of a call with too few tiles to fill the GPU with pairs) the two
+// softmax streams take alternate blocks of the same rows, and their results are joined in place:
+// both streams' accumulators of a row lie in the same lane of tensor memory.  Either way two
+// streams are in flight, and while one is in its softmax the other's products run.
 //
 // Split.  All blocks of all units lie on one line (request, KV head, tile, block) that is cut into
-// equal parts, one per CTA: no tail wave whatever the lengths.  A unit that a cut falls into
-// leaves unnormalised partial results (fp32) in the workspace, and the CTA that arrives last joins
-// them in the order of the parts, so the result does not depend on timing.  Every CTA works its
-// part out from the lengths by itself; there is no planning launch, and no CTA waits for another.
+// equal parts, one per CTA: no tail wave whatever the lengths.  Every CTA works its part out from
+// the lengths by itself; no CTA waits for another.  A unit that a cut falls into leaves
+// unnormalised fp32 results in the workspace, and a second small kernel joins them in the order of
+// the parts, so the result does not depend on timing.
 //
 // Roles of a CTA (one per SM):
 //   warps 0-3 / 4-7  softmax streams 0 / 1, one thread per row: scores from tensor memory, running
@@ -50,12 +51,20 @@ constexpr int kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;
 constexpr int kThreads = 384;
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // 256 * 216 + 128 * 72 = 384 * 168
-constexpr int kMinBlocks = 4;              // fewest blocks worth a CTA of their own
+constexpr int kUnitCells = 1;              // what a unit costs beside its blocks, in blocks
+constexpr int kMinCells = 3;               // least work worth a CTA of its own, where units are long
+constexpr int kJoinRows = 16;              // rows of a unit that a block of the second kernel joins
 constexpr int kTmemCols = 512;             // S0 S1 O0 O1; the weights lie over the scores
 constexpr int kRowWarps = 8;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
-// A slot of the workspace: one part's unnormalised results, two streams of 128 rows.
+// The workspace: a list of the units that were cut (entry c: the one that begins in CTA c's part
+// and ends behind it), then two slots a CTA for a part's unnormalised results, 256 rows each.
+struct Cut {
+  int parts, kh, tok0, ntok;
+};
+constexpr int kMaxCtas = 1024;
+constexpr int64_t kCutBytes = kMaxCtas * static_cast<int64_t>(sizeof(Cut));
 constexpr int64_t kSlotFloats = 2 * kRows * 128;
 constexpr int64_t kSlotBytes = kSlotFloats * 4 + 2 * kRows * 8;
 
@@ -73,7 +82,7 @@ struct Item {
   int k0, khi;             // keys [k0, khi) are attended by some row of the unit
   int blk0, nblk;          // this part's blocks, counted from k0
   int qbuf;                // query buffer of a single unit
-  int parts, cta0;         // CTAs that share the unit, the first of them
+  int parts;               // CTAs that share the unit
   int slot;
   unsigned nonfinite;      // a value that only some rows attend was infinite or NaN
 };
@@ -88,13 +97,13 @@ struct Control {
   int start_b;
   uint32_t tmem;
   unsigned abort;
-  unsigned last;
+  float2 ml[2][kRows];     // a single unit's maxima and sums, by stream
 };
 
 constexpr int kSmemQ = 0;
 constexpr int kSmemKv = 2 * kTileBytes;
 constexpr int kSmemControl = kSmemKv + kStages * kTileBytes;
-constexpr int kSmemBytes = kSmemControl + static_cast<int>(sizeof(Control)) + 1024;   // + alignment
+constexpr int kSmemBytes = kSmemControl + static_cast<int>(sizeof(Control));
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -279,10 +288,11 @@ struct Unit {
   int t0, ntok;            // tokens of the request
   int k0, khi, nblk;
 };
-__device__ __forceinline__ Unit unit_of(const Request& r, int window, int tile_tokens, int t) {
+// `span`: tokens of a whole unit (one or two tiles)
+__device__ __forceinline__ Unit unit_of(const Request& r, int window, int span, int t) {
   Unit u;
-  u.t0 = t * 2 * tile_tokens;
-  u.ntok = min(2 * tile_tokens, r.n - u.t0);
+  u.t0 = t * span;
+  u.ntok = min(span, r.n - u.t0);
   const int p0 = r.kv - r.n + u.t0;
   u.khi = max(0, p0 + u.ntok);
   u.k0 = 0;
@@ -290,15 +300,34 @@ __device__ __forceinline__ Unit unit_of(const Request& r, int window, int tile_t
   u.nblk = window == 0 || u.k0 >= u.khi ? 0 : (u.khi - u.k0 + kBlk - 1) / kBlk;
   return u;
 }
-__device__ __forceinline__ int units_of(const Request& r, int tile_tokens) {
-  return (r.n + 2 * tile_tokens - 1) / (2 * tile_tokens);
-}
-// length of one KV head of a request on the line: its blocks, 1 for a unit without keys
-__device__ __forceinline__ long long head_length(const Request& r, int window, int tile_tokens) {
+// Cells of a unit on the line: what it costs beside its blocks, then its blocks.
+__device__ __forceinline__ int cells_of(const Unit& u) { return kUnitCells + u.nblk; }
+__device__ __forceinline__ long long head_cells(const Request& r, int window, int span) {
   long long c = 0;
-  const int nt = units_of(r, tile_tokens);
-  for (int t = 0; t < nt; ++t) c += max(1, unit_of(r, window, tile_tokens, t).nblk);
+  for (int t = 0; t * span < r.n; ++t) c += cells_of(unit_of(r, window, span, t));
   return c;
+}
+
+// Sum over the CTA of `mine`; `before` gets what the threads before this one hold.
+__device__ __forceinline__ long long scan_cta(long long mine, long long& before, long long* warps) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += o;
+  }
+  __syncthreads();
+  if (lane == 31) warps[warp] = x;
+  __syncthreads();
+  long long total = 0;
+  before = x - mine;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += warps[w];
+    total += warps[w];
+  }
+  return total;
 }
 
 // The ring position of block `blk`'s K and V within a unit: K and V in turn when both streams use
@@ -341,41 +370,43 @@ __device__ __forceinline__ const void* v_row(const MacB200ChunkArgs& a, const It
 // ------------------------------------------------------------------------------------ the kernel
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtensorMap q_map) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];      // the swizzle repeats every 1024 bytes
   Control& ctl = *reinterpret_cast<Control*>(smem + kSmemControl);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.Hq / a.Hkv;
   const int tile_tokens = kRows / G;
+  Cut* const cuts = static_cast<Cut*>(a.workspace);
 
   // ---- the line: this CTA's part of it, and the request that the part begins in
   const int per = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  long long mine = 0;
+  long long mine = 0, before;
   for (int b = b0; b < b1; ++b)
-    mine += a.Hkv * head_length(load_request(a, b, blockIdx.x == 0), a.window, tile_tokens);
-  long long before = mine;                               // inclusive within the warp, then exclusive
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before += o;
+    mine += a.Hkv * static_cast<long long>((load_request(a, b, blockIdx.x == 0).n + tile_tokens - 1) / tile_tokens);
+  // pairs of tiles once there are enough of them for every CTA
+  const int span = scan_cta(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
+  long long units = 0;
+  mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Request r = load_request(a, b, false);
+    mine += a.Hkv * head_cells(r, a.window, span);
+    units += a.Hkv * static_cast<long long>((r.n + span - 1) / span);
   }
-  if (lane == 31) ctl.scan[warp] = before;
-  __syncthreads();
-  long long total = 0;
-  before -= mine;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += ctl.scan[w];
-    total += ctl.scan[w];
+  long long unused;
+  units = scan_cta(units, unused, ctl.scan);
+  const long long total = scan_cta(mine, before, ctl.scan);
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(units, total / kMinCells)));
+  if (tid == 0) cuts[blockIdx.x].parts = 0;
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
+  if ((smem_u32(smem) & 1023u) != 0u) {                  // the operand layout would not hold
+    if (tid == 0) atomicOr(&g_chunk_status, MAC_B200_STATUS_SCHED_OVERFLOW);
+    return;
   }
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1ll, total / kMinBlocks)));
-  if (total == 0 || static_cast<int>(blockIdx.x) >= ctas) return;
   const long long lo = total * blockIdx.x / ctas, hi = total * (blockIdx.x + 1) / ctas;
   if (lo >= before && lo < before + mine) {
     long long at = before;
     for (int b = b0; b < b1; ++b) {
-      const long long len = a.Hkv * head_length(load_request(a, b, false), a.window, tile_tokens);
+      const long long len = a.Hkv * head_cells(load_request(a, b, false), a.window, span);
       if (lo < at + len) {
         ctl.start_b = b;
         ctl.start_pos = at;
@@ -430,7 +461,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       const uint32_t q_bytes = static_cast<uint32_t>(tile_tokens) * G * 128u;   // of one 64-dim half
       while (ok && cur < hi) {
         const Request r = load_request(a, b, false);
-        const long long len = r.n > 0 ? head_length(r, a.window, tile_tokens) : 0;
+        const long long len = head_cells(r, a.window, span);
         if (cur >= req_pos + len * a.Hkv) {
           req_pos += len * a.Hkv;
           ++b;
@@ -438,36 +469,52 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         }
         int kh = static_cast<int>((cur - req_pos) / len), t = 0;
         long long u0 = req_pos + kh * len;
-        Unit u = unit_of(r, a.window, tile_tokens, 0);
-        while (cur >= u0 + max(1, u.nblk)) {
-          u0 += max(1, u.nblk);
-          u = unit_of(r, a.window, tile_tokens, ++t);
+        Unit u = unit_of(r, a.window, span, 0);
+        while (cur >= u0 + cells_of(u)) {
+          u0 += cells_of(u);
+          u = unit_of(r, a.window, span, ++t);
         }
-        const int nt = units_of(r, tile_tokens);
         while (ok && cur < hi && kh < a.Hkv) {
-          const long long u1 = u0 + max(1, u.nblk);
-          const long long end = min(hi, u1);
+          const Unit now = u;
+          const long long first = u0 + kUnitCells, u1 = u0 + cells_of(now);
+          const long long from = max(cur, first), to = min(hi, u1);
+          const int tok0 = r.row0 + now.t0, head = kh;
+          const bool begins = cur <= u0;
+          cur = max(cur, to);
+          u0 = u1;
+          if (++t * span >= r.n) {
+            t = 0;
+            ++kh;
+          }
+          u = unit_of(r, a.window, span, t);
+          if (now.nblk > 0 ? from >= to : !begins) continue;   // no block of it in this part
           const int slot = it & (kItems - 1);
-          ok = ok && mbar_wait(&ctl.item_empty[slot], (it / kItems) + 1, abort_flag);
+          ok = mbar_wait(&ctl.item_empty[slot], (it / kItems) + 1, abort_flag);
           if (!ok) break;
           Item& o = ctl.items[slot];
           o.valid = 1;
-          o.dual = u.ntok > tile_tokens;
-          o.kh = kh;
+          o.dual = now.ntok > tile_tokens;
+          o.kh = head;
           o.req = r.req;
-          o.tok0 = r.row0 + u.t0;
-          o.ntok = u.ntok;
-          o.pos0 = r.kv - r.n + u.t0;
-          o.k0 = u.k0;
-          o.khi = u.khi;
-          o.blk0 = static_cast<int>(cur - u0);
-          o.nblk = u.nblk == 0 ? 0 : static_cast<int>(end - cur);
+          o.tok0 = tok0;
+          o.ntok = now.ntok;
+          o.pos0 = r.kv - r.n + now.t0;
+          o.k0 = now.k0;
+          o.khi = now.khi;
+          o.blk0 = static_cast<int>(from - first);
+          o.nblk = now.nblk == 0 ? 0 : static_cast<int>(to - from);
           o.qbuf = toggle;
-          o.cta0 = static_cast<int>(((u0 + 1) * ctas - 1) / total);
-          o.parts = static_cast<int>((u1 * ctas - 1) / total) - o.cta0 + 1;
-          o.slot = 2 * static_cast<int>(blockIdx.x) + (o.cta0 == static_cast<int>(blockIdx.x) ? 1 : 0);
+          o.parts = 1;
+          o.slot = 0;
+          if (now.nblk > 0) {                            // the CTAs of its first and last block
+            const int cta0 = static_cast<int>(((first + 1) * ctas - 1) / total);
+            o.parts = static_cast<int>((u1 * ctas - 1) / total) - cta0 + 1;
+            const bool first_part = cta0 == static_cast<int>(blockIdx.x);
+            o.slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 1 : 0);
+            if (first_part && o.parts > 1) cuts[blockIdx.x] = Cut{o.parts, head, tok0, now.ntok};
+          }
           o.nonfinite = 0u;
-          const int dual = o.dual, tok0 = o.tok0, nblk = o.nblk;
+          const int dual = o.dual, nblk = o.nblk;
           mbar_arrive(&ctl.item_full[slot]);
           if (nblk > 0) {
             for (int i = 0; i < (dual ? 2 : 1) && ok; ++i) {
@@ -477,19 +524,12 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
               ++q_uses[buf];
               mbar_expect_tx(&ctl.q_full[buf], 2 * q_bytes);
               const uint32_t dst = smem_u32(smem + kSmemQ + buf * kTileBytes);
-              tma_load_3d(dst, &q_map, 0, kh * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
-              tma_load_3d(dst + kHalfBytes, &q_map, 64, kh * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
+              tma_load_3d(dst, &q_map, 0, head * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
+              tma_load_3d(dst + kHalfBytes, &q_map, 64, head * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
             }
             if (!dual) toggle ^= 1;
           }
           ++it;
-          cur = end;
-          u0 = u1;
-          if (++t == nt) {
-            t = 0;
-            ++kh;
-          }
-          u = unit_of(r, a.window, tile_tokens, t);
         }
       }
       const int slot = it & (kItems - 1);
@@ -636,9 +676,8 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     const uint32_t t_s = tmem + s * 128 + t_lane, t_o = tmem + 256 + s * 128 + t_lane;
     const float scale = a.sm_scale * 1.4426950408889634f;
     const float slack = 8.f / scale;                     // scores may exceed the kept maximum by this
-    char* const slots = static_cast<char*>(a.workspace) + 4096;
-    unsigned* const counters = static_cast<unsigned*>(a.workspace);
-    uint32_t s_uses = 0, o_uses = 0, j_uses = 0, pos = 0;
+    char* const slots = static_cast<char*>(a.workspace) + kCutBytes;
+    uint32_t s_uses = 0, o_uses[2] = {0, 0}, j_uses = 0, pos = 0;
     bool ok = true;
     auto both_streams = [&]() {                          // barrier of the eight softmax warps, bounded
       __syncwarp();
@@ -760,38 +799,61 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       }
       if (!ok) break;
       pos += 2 * nblk;
-      const bool worked = blk_first < nblk;
-      if (worked) {
-        ok = mbar_wait(&ctl.o_full[s], o_uses, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        ++o_uses;
-        tc_fence_after();
+      // ---- the unit's (part's) result.  Dual: a thread's own row.  Single: both streams hold a share
+      // of every row; stream 0 finishes dims 0-63 and stream 1 dims 64-127.
+      const int phases[2] = {nblk > 0 ? 1 : 0, nblk > (dual ? 0 : 1) ? 1 : 0};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (phases[i] && (!dual || i == s)) ok = ok && mbar_wait(&ctl.o_full[i], o_uses[i], abort_flag);
+        o_uses[i] += phases[i];
       }
-      const bool join = o.parts > 1 || (!dual && nblk > 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      float fa = 1.f, fb = 0.f;                          // what the accumulators are multiplied by
+      if (!dual) {
+        ctl.ml[s][r] = make_float2(m, l);
+        ok = both_streams();
+        if (!ok) break;
+        const float2 x = ctl.ml[0][r], y = ctl.ml[1][r];
+        m = fmaxf(x.x, y.x);
+        fa = x.x == -INFINITY ? 0.f : ex2((x.x - m) * scale);
+        fb = y.x == -INFINITY ? 0.f : ex2((y.x - m) * scale);
+        // a NaN sum has to survive a maximum of -inf (every logit NaN)
+        l = (x.y == 0.f ? 0.f : x.x == -INFINITY ? x.y : x.y * fa) +
+            (y.y == 0.f ? 0.f : y.x == -INFINITY ? y.y : y.y * fb);
+      }
+      tc_fence_after();
       __threadfence_block();
-      const bool refill = worked && *reinterpret_cast<volatile unsigned*>(&o.nonfinite) != 0u;
-      const int hq = o.kh * G + r % G;
-      const int64_t orow = static_cast<int64_t>(o.tok0 + t) * a.Hq + hq;
-      const bool direct = !join && live && (dual || s == 0);
+      const bool refill = *reinterpret_cast<volatile unsigned*>(&o.nonfinite) != 0u;
+      const bool cut = o.parts > 1;
+      const int64_t orow = static_cast<int64_t>(o.tok0 + t) * a.Hq + o.kh * G + r % G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float* part = reinterpret_cast<float*>(slots + static_cast<int64_t>(o.slot) * kSlotBytes);
-      if (any_live && (worked || direct)) {
+      float* const part = reinterpret_cast<float*>(slots + static_cast<int64_t>(o.slot) * kSlotBytes);
+      const int prow = dual ? s * kRows + r : r;
+      const uint32_t t_a = dual ? t_o : tmem + 256 + t_lane;
+      if (any_live) {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = dual ? 0 : 2 * s; c < (dual ? 4 : 2 * s + 2); ++c) {
           float v[32];
-          if (worked) {
+          if (nblk > 0) {
             uint32_t w[32];
-            tmem_ld32(t_o + c * 32, w);
+            tmem_ld32(t_a + c * 32, w);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]);
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]) * fa;
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
+          if (!dual && nblk > 1) {
+            uint32_t w[32];
+            tmem_ld32(t_a + 128 + c * 32, w);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = fmaf(__uint_as_float(w[i]), fb, v[i]);
+          }
           if (refill && live) {
-            for (int blk = blk_first; blk < nblk; blk += step) {
+            for (int blk = 0; blk < nblk; ++blk) {
               const int kb = first + blk * kBlk;
               if (!partly_attended(o, a.window, kb)) continue;
               for (int key = max(kb, key_lo); key < min(kb + kBlk, key_hi); ++key) {
@@ -806,7 +868,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
               }
             }
           }
-          if (direct) {
+          if (live && !cut) {
             uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + orow * 256 + c * 64);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -816,70 +878,23 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
                 w[j] = l == 0.f ? 0u : pack_bf16(v[i * 8 + 2 * j] * inv, v[i * 8 + 2 * j + 1] * inv);
               dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          } else if (live && join) {
-            float4* dst = reinterpret_cast<float4*>(part + (s * kRows + r) * 128 + c * 32);
+          } else if (live) {
+            float4* dst = reinterpret_cast<float4*>(part + prow * 128 + c * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              __stcg(dst + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+              dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         }
       }
-      if (direct && a.lse)
-        a.lse[orow] = l == 0.f ? -INFINITY : (m * scale + log2f(l)) * 0.6931471805599453f;
-      if (join) {
-        if (live)
-          __stcg(reinterpret_cast<float2*>(part + kSlotFloats) + s * kRows + r, make_float2(m, l));
-        __threadfence();
-        ok = both_streams();
-        if (!ok) break;
-        if (tid == 0) {
-          ctl.last = o.parts == 1 || atomicInc(counters + o.cta0, o.parts - 1) == static_cast<unsigned>(o.parts - 1);
-          __threadfence();
-        }
-        ok = both_streams();
-        if (!ok) break;
-        if (ctl.last) {
-          // ---- join the parts of this unit: one warp a row, four dims a lane
-          const int rows = ntok * G;
-          const int per_part = dual ? 1 : 2;
-          for (int row = warp; row < rows; row += kSoftmaxWarps) {
-            const int token = row / G, g = row - token * G;
-            const int str = dual && token >= tile_tokens;
-            const int rr = str ? row - tile_tokens * G : row;
-            auto slot_of = [&](int i) {                  // contribution i: part i / per_part, stream
-              const int c = o.cta0 + i / per_part;
-              return slots + static_cast<int64_t>(2 * c + (c == o.cta0 ? 1 : 0)) * kSlotBytes;
-            };
-            auto lane_of = [&](int i) { return (dual ? str : i & 1) * kRows + rr; };
-            const int n = o.parts * per_part;
-            float mx = -INFINITY;
-            for (int i = lane; i < n; i += 32)
-              mx = fmaxf(mx, __ldcg(reinterpret_cast<const float2*>(slot_of(i) + kSlotFloats * 4) + lane_of(i)).x);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float ms = mx == -INFINITY ? 0.f : mx * scale;
-            float lsum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-              const char* sl = slot_of(i);
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(sl + kSlotFloats * 4) + lane_of(i));
-              if (ml.y == 0.f) continue;                 // nothing attended in this part
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(sl) + lane_of(i) * 32 + lane);
-              const float f = ex2(ml.x * scale - ms);
-              lsum += ml.y * f;
-              acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
-            }
-            const float k = lsum == 0.f ? 0.f : 1.f / lsum;
-            const int64_t to = static_cast<int64_t>(o.tok0 + token) * a.Hq + o.kh * G + g;
-            uint2 w = make_uint2(0u, 0u);
-            if (lsum != 0.f) w = make_uint2(pack_bf16(acc.x * k, acc.y * k), pack_bf16(acc.z * k, acc.w * k));
-            *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + to * 256 + lane * 8) = w;
-            if (a.lse && lane == 0)
-              a.lse[to] = lsum == 0.f ? -INFINITY : (ms + log2f(lsum)) * 0.6931471805599453f;
-          }
-        }
-        ok = both_streams();                             // the slot and ctl.last are free again
+      if (live && (dual || s == 0)) {
+        if (cut)
+          reinterpret_cast<float2*>(part + kSlotFloats)[prow] = make_float2(m, l);
+        else if (a.lse)
+          a.lse[orow] = l == 0.f ? -INFINITY : (m * scale + log2f(l)) * 0.6931471805599453f;
+      }
+      if (!dual) {
+        tc_fence_before();
+        ok = both_streams();                             // the accumulators and ctl.ml are free again
         if (!ok) break;
       }
       __syncwarp();
@@ -893,6 +908,76 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------- units that were cut
+// Block (c, y) joins rows [16 y, 16 y + 16) of the unit that begins in part c.  A row's parts are
+// shared by as many of the eight warps as the rows leave free; four dims a lane.  The sums run in
+// an order that the parts alone decide.
+__global__ void __launch_bounds__(256)
+chunk_join_kernel(const MacB200ChunkArgs a) {
+  const Cut cut = static_cast<const Cut*>(a.workspace)[blockIdx.x];
+  const int G = a.Hq / a.Hkv, tile_tokens = kRows / G;
+  const int row_first = blockIdx.y * kJoinRows, rows = min(cut.ntok * G - row_first, kJoinRows);
+  if (cut.parts == 0 || rows <= 0) return;
+  __shared__ float4 acc_s[8][32];
+  __shared__ float l_s[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;   // warps of a row
+  const char* const slots = static_cast<const char*>(a.workspace) + kCutBytes;
+  const float scale = a.sm_scale * 1.4426950408889634f;
+  const bool dual = cut.ntok > tile_tokens;
+  for (int rr = warp / share; rr < kJoinRows; rr += 8 / share) {
+    const bool live = rr < rows;
+    if (share == 1 && !live) break;
+    const int row = row_first + (live ? rr : 0);
+    const int token = row / G, g = row - token * G;
+    const int at = dual && token >= tile_tokens ? row - tile_tokens * G + kRows : row;
+    auto slot_of = [&](int i) {
+      return slots + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kSlotBytes;
+    };
+    float mx = -INFINITY;
+    for (int i = lane; i < cut.parts; i += 32)
+      mx = fmaxf(mx, reinterpret_cast<const float2*>(slot_of(i) + kSlotFloats * 4)[at].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float ms = mx == -INFINITY ? 0.f : mx * scale;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = warp % share; i < cut.parts; i += share) {
+      const char* sl = slot_of(i);
+      const float2 ml = reinterpret_cast<const float2*>(sl + kSlotFloats * 4)[at];
+      const float4 x = reinterpret_cast<const float4*>(sl)[at * 32 + lane];
+      if (ml.y != 0.f) {                                 // something attended in this part
+        const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x * scale - ms);   // NaN sums stay
+        l += ml.y * f;
+        acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
+      }
+    }
+    if (share > 1) {
+      acc_s[warp][lane] = acc;
+      if (lane == 0) l_s[warp] = l;
+      __syncthreads();
+      if (warp % share == 0)
+        for (int w = 1; w < share; ++w) {
+          const float4 x = acc_s[warp + w][lane];
+          l += l_s[warp + w];
+          acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+        }
+      __syncthreads();
+    }
+    if (live && warp % share == 0) {
+      const float k = l == 0.f ? 0.f : 1.f / l;
+      const int64_t to = static_cast<int64_t>(cut.tok0 + token) * a.Hq + cut.kh * G + g;
+      uint2 w = make_uint2(0u, 0u);
+      if (l != 0.f) w = make_uint2(pack_bf16(acc.x * k, acc.y * k), pack_bf16(acc.z * k, acc.w * k));
+      *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + to * 256 + lane * 8) = w;
+      if (a.lse && lane == 0)
+        a.lse[to] = l == 0.f ? -INFINITY : (ms + log2f(l)) * 0.6931471805599453f;
+    }
+    if (share > 1) break;                                // 8 / share rows cover them all
   }
 }
 
@@ -969,8 +1054,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const MacB20
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// counters (one a CTA), then two slots a CTA
-int64_t workspace_bytes(int sms) { return 4096 + 2 * static_cast<int64_t>(sms) * kSlotBytes; }
+int64_t workspace_bytes(int sms) { return kCutBytes + 2 * static_cast<int64_t>(sms) * kSlotBytes; }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -1037,7 +1121,7 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
     MAC_REQUIRE(blocks < (int64_t(1) << 31), "chunk problem too large");
     chunk_rows_kernel<true><<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, stream>>>(a);
   } else {
-    MAC_REQUIRE(sms <= 1024, "too many multiprocessors");
+    MAC_REQUIRE(sms <= kMaxCtas, "too many multiprocessors");
     if (const int rc = prepare_kernel(device)) return rc;
     EncodeTiledFn enc = encode_tiled_fn();
     if (enc == nullptr) return fail(MAC_B200_EUNSUPPORTED, "cuTensorMapEncodeTiled is not available");
@@ -1052,6 +1136,9 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
                       CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return fail(MAC_B200_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
     chunk_attention_kernel<<<sms, kThreads, kSmemBytes, stream>>>(a, q_map);
+    MAC_CUDA(cudaGetLastError());
+    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+    chunk_join_kernel<<<dim3(sms, 2 * kRows / kJoinRows), 256, 0, stream>>>(a);
   }
   MAC_CUDA(cudaGetLastError());
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
