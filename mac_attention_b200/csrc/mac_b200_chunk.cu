@@ -20,9 +20,9 @@
 // Roles of a CTA (one per SM):
 //   warps 0-3 / 4-7  softmax streams 0 / 1, one thread per row: scores from tensor memory, running
 //                    maximum and sum in fp32, bf16 weights back over the scores, results out
-//   warp 8           issues the products: S = Q K^T from shared memory, O += P V with P read from
+//   warps 8, 9       issue the streams' products: S = Q K^T from shared memory, O += P V with P from
 //                    tensor memory and V from the rows as they lie in the pool (keys x dims)
-//   warps 9, 11      fetch K/V rows by the page table into the swizzled operand layout (cp.async)
+//   warps 12-15      fetch K/V rows by the page table into the swizzled operand layout (cp.async)
 //   warp 10          works out the units of this CTA's part, fetches the query tiles
 // The running maximum is kept until a row's scores exceed it by 2^8 in weight: the rescaling of O
 // is rare, and exact when it happens.  Weights are rounded to bf16 for the second product (the
@@ -43,14 +43,16 @@ namespace {
 
 constexpr int kBlk = 128;                  // keys of a block
 constexpr int kRows = 128;                 // rows of a tile
+constexpr int kHalf = 64;                  // keys of a step: what a stream takes from scores to weights at once
 constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 bf16 in the 128-byte-swizzled layout
 constexpr int kTileBytes = 2 * kHalfBytes;
 constexpr int kStages = 5;                 // K/V blocks in shared memory
 constexpr int kItems = 4;                  // units announced ahead
 constexpr int kSoftmaxWarps = 8;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kPlanWarp = 10;
-constexpr int kThreads = 384;
-constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // 256 * 216 + 128 * 72 = 384 * 168
+constexpr int kMmaWarp = 8, kPlanWarp = 10, kLoadWarp = 12, kLoadWarps = 4;
+constexpr int kThreads = 512;
+// registers a thread after the warpgroups have traded theirs: 256 * 152 + 128 * 96 + 128 * 112 = 512 * 128
+constexpr int kSoftmaxRegs = 152, kControlRegs = 96, kLoadRegs = 112;
 constexpr int kUnitCells = 1;              // what a unit costs beside its blocks, in blocks
 constexpr int kMinCells = 3;               // least work worth a CTA of its own, where units are long
 constexpr int kJoinRows = 16;              // rows of a unit that a block of the second kernel joins
@@ -65,12 +67,15 @@ struct Cut {
 };
 constexpr int kMaxCtas = 1024;
 constexpr int64_t kCutBytes = kMaxCtas * static_cast<int64_t>(sizeof(Cut));
-constexpr int64_t kSlotFloats = 2 * kRows * 128;
-constexpr int64_t kSlotBytes = kSlotFloats * 4 + 2 * kRows * 8;
+constexpr int kSlotRows = 2 * kRows;
+constexpr int64_t kSlotFloats = kSlotRows * 128;       // [four dims][row]: a warp stores whole lines
+constexpr int64_t kSlotBytes = kSlotFloats * 4 + kSlotRows * 8;   // then (maximum, sum) of each row
 
-// bf16 x bf16 -> fp32, M 128, N 128; the second product's B operand is dim-contiguous
-constexpr uint32_t kIdescQk = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-constexpr uint32_t kIdescPv = kIdescQk | (1u << 16);
+// bf16 x bf16 -> fp32, M 128: N 64 keys of the first product; N 128 dims of the second, whose B
+// operand is dim-contiguous
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescQk = kIdesc | ((64u >> 3) << 17);
+constexpr uint32_t kIdescPv = kIdesc | ((128u >> 3) << 17) | (1u << 16);
 
 __device__ unsigned g_chunk_status = 0;
 
@@ -89,7 +94,7 @@ struct Item {
 
 struct Control {
   uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2];
   uint64_t item_full[kItems], item_empty[kItems], join;
   Item items[kItems];
   long long scan[kThreads / 32];
@@ -138,11 +143,12 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 // Waits for the phase of `count` earlier phases.  False when the limit ran out here or in another
 // warp of the CTA: the caller leaves its loop.
 __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, unsigned* abort_flag) {
-  const unsigned long long t0 = now_ns();
+  unsigned long long t0 = 0;                             // the clock is slow to read: not before it is needed
   for (unsigned spins = 1;; ++spins) {
-    if (mbar_try(bar, parity)) return true;            // each try may itself block for a while
-    if ((spins & 31u) == 0u) {
+    if (mbar_try(bar, parity)) return true;              // each try may itself block for a while
+    if ((spins & 63u) == 0u) {
       if (*reinterpret_cast<volatile unsigned*>(abort_flag) != 0u) return false;
+      if (t0 == 0) t0 = now_ns();
       if (now_ns() - t0 > kWaitLimitNs) {
         *reinterpret_cast<volatile unsigned*>(abort_flag) = 1u;
         atomicOr(&g_chunk_status, MAC_B200_STATUS_COPY_TIMEOUT);
@@ -170,7 +176,7 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead) {
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
          (static_cast<uint64_t>(2) << 61);
 }
-// D (+)= A B^T, 128 x 128 x 16: A and B from shared memory
+// D (+)= A B^T, 128 x 64 x 16: A and B from shared memory
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -207,6 +213,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// ties loaded registers to the wait before it: nothing that uses them may move above it
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -234,9 +245,40 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the largest of three, NaN if any is NaN
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+// a load that stays where it is written: ahead of its use
+__device__ __forceinline__ int load_early(const int32_t* p) {
+  int v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
 }
 // 16 bytes, or 16 zeros when `bytes` is 0
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -258,6 +300,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+
+// a value that every lane holds alike, so that the compiler knows it
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
 }
 
 // ---------------------------------------------------------------------------- units on the line
@@ -372,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtensorMap q_map) {
   extern __shared__ __align__(1024) uint8_t smem[];      // the swizzle repeats every 1024 bytes
   Control& ctl = *reinterpret_cast<Control*>(smem + kSmemControl);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int G = a.Hq / a.Hkv;
   const int tile_tokens = kRows / G;
   Cut* const cuts = static_cast<Cut*>(a.workspace);
@@ -419,19 +471,21 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   // ---- barriers, tensor memory
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&ctl.kv_full[i], 64);
-      mbar_init(&ctl.kv_empty[i], 1);
+      mbar_init(&ctl.kv_full[i], kLoadWarps * 32);
+      mbar_init(&ctl.kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.q_full[i], 1);
-      mbar_init(&ctl.q_empty[i], 1);
-      mbar_init(&ctl.s_full[i], 1);
-      mbar_init(&ctl.p_full[i], 4);
-      mbar_init(&ctl.o_full[i], 1);
+      mbar_init(&ctl.q_empty[i], 2);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&ctl.s_full[i][h], 1);
+        mbar_init(&ctl.p_full[i][h], 4);
+        mbar_init(&ctl.o_done[i][h], 1);
+      }
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&ctl.item_full[i], 1);
-      mbar_init(&ctl.item_empty[i], kSoftmaxWarps + 3);
+      mbar_init(&ctl.item_empty[i], kSoftmaxWarps + kLoadWarps + 2);
     }
     mbar_init(&ctl.join, kSoftmaxWarps);
     ctl.abort = 0u;
@@ -446,11 +500,82 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem;
+  const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(ctl.tmem)));
   unsigned* const abort_flag = &ctl.abort;
 
-  if (warp >= kSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp >= kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    // ---- K/V rows by the page table: sixteen lanes fetch a row, a warp 32 of a block's 128
+    const int part = (warp - kLoadWarp) * 32;
+    const int sub = lane >> 4, chunk = lane & 15;
+    const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 256;
+    uint32_t to[4];                                    // where this lane's chunk goes in rows 2i + sub
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = part + 2 * i + sub;
+      to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
+              (((chunk & 7) ^ (row & 7)) << 4);
+    }
+    uint32_t pos = 0;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int slot = it & (kItems - 1);
+      ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const Item& o = ctl.items[slot];
+      if (!o.valid) break;
+      const int dual = o.dual, nblk = o.nblk, khi = o.khi;
+      const int first = o.k0 + o.blk0 * kBlk;
+      const int64_t col = o.kh * 256 + chunk * 16;
+      const int32_t* table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
+      // Key `lane` of this warp's part of ring position i: the key, and what the table says of it.
+      // Table entries are asked for two positions ahead and looked at when they are needed.
+      struct Entry {
+        int key, row;
+        bool is_v;
+      };
+      auto entry_of = [&](int i) {
+        Entry e{khi, 0, false};
+        if (i >= 2 * nblk) return e;
+        int blk;
+        ring_at(dual, nblk, i, blk, e.is_v);
+        e.key = first + blk * kBlk + part + lane;
+        if (e.key < khi) e.row = load_early(table + e.key);
+        return e;
+      };
+      Entry next = entry_of(0), after = entry_of(1);
+      for (int i = 0; i < 2 * nblk; ++i, ++pos) {
+        const Entry e = next;
+        next = after;
+        after = entry_of(i + 2);
+        const bool is_v = e.is_v;
+        const int st = pos % kStages;
+        ok = mbar_wait(&ctl.kv_empty[st], pos / kStages + 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const char* src = static_cast<const char*>(is_v ? a.v : a.k) + col;
+        int row = -1;                                    // no key: arrives as zeros
+        if (e.key < khi) {
+          if (e.row >= 0 && e.row < a.kv_tokens)
+            row = e.row;
+          else
+            atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int tok = __shfl_sync(0xffffffffu, row, 2 * j + sub);
+          cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes,
+                     src + (tok < 0 ? 0 : tok) * row_stride, tok < 0 ? 0 : 16);
+        }
+        cp_async_arrive(&ctl.kv_full[st]);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");   // nothing in flight when the CTA leaves
+  } else if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
 
     if (warp == kPlanWarp && lane == 0) {
       // ---- the units of this part, in order, and their query tiles
@@ -544,127 +669,124 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           while (q_uses[i] > 0 && !mbar_try(smem_u32(&ctl.q_full[i]), (q_uses[i] - 1) & 1u) &&
                  now_ns() - t0 < kWaitLimitNs) {}
         }
-    } else if (warp == kLoadWarp || warp == kLoadWarp + 2) {
-      // ---- K/V rows by the page table: sixteen lanes fetch a row, a warp 64 of a block's 128
-      const int half = warp == kLoadWarp ? 0 : 64;
-      const int sub = lane >> 4, chunk = lane & 15;
-      const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 256;
-      uint32_t to[4];                                    // where this lane's chunk goes in rows 2i + sub
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = half + 2 * i + sub;
-        to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
-                (((chunk & 7) ^ (row & 7)) << 4);
-      }
-      uint32_t pos = 0;
+    } else if (warp < kMmaWarp + 2) {
+      // ---- the products of stream `warp - kMmaWarp`.  The whole warp walks through the steps and one
+      // lane issues: in code that the compiler knows to be uniform the operands' descriptors stay in
+      // uniform registers (a lane that branched off by itself took 90 cycles an instruction).  One
+      // warp a stream: neither waits for the other's softmax.
+      const int s = warp - kMmaWarp;
+      const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
+      uint32_t pos = 0, seen = 0, q_uses[2] = {0u, 0u};
+      uint32_t t_qk = 0, t_pv = 0;                       // steps of 64 keys issued so far
       bool ok = true;
+      int dual = 0, nblk = 0;
+      // A barrier tells its phases apart by one bit, so no phase may pass a waiter by: both streams'
+      // warps wait for every ring position in order, and each gives every position back -- with its
+      // last product on it, or at once when the block is the other stream's.  The same for query
+      // tiles.
+      auto have = [&](uint32_t p) {
+        bool good = true;
+        for (; good && seen <= p; ++seen) {
+          good = mbar_wait(&ctl.kv_full[seen % kStages], seen / kStages, abort_flag);
+          if (!dual) {
+            int blk;
+            bool is_v;
+            ring_at(0, nblk, static_cast<int>(seen - pos), blk, is_v);
+            if ((blk & 1) != s && lane == 0) mbar_arrive(&ctl.kv_empty[seen % kStages]);
+          }
+        }
+        return __all_sync(0xffffffffu, good) != 0;
+      };
       for (int it = 0; ok; ++it) {
         const int slot = it & (kItems - 1);
         ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const Item& o = ctl.items[slot];
-        if (!o.valid) break;
-        const int dual = o.dual, nblk = o.nblk, khi = o.khi;
-        const int first = o.k0 + o.blk0 * kBlk;
-        const int64_t col = o.kh * 256 + chunk * 16;
-        const int32_t* table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
+        if (!uniform(o.valid)) break;
+        dual = uniform(o.dual);
+        nblk = uniform(o.nblk);
+        const int qbuf = uniform(o.qbuf), keys = uniform(o.khi - o.k0 - o.blk0 * kBlk);
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
-        // pool rows of keys `lane` and 32 + `lane` of this warp's half; -1: no key, arrives as zeros
-        auto rows_of = [&](int i, int (&row)[2], bool& is_v) {
-          int blk;
-          ring_at(dual, nblk, i, blk, is_v);
-          const int key = first + blk * kBlk + half + lane;
-          row[0] = key < khi ? __ldg(table + key) : -1;
-          row[1] = key + 32 < khi ? __ldg(table + key + 32) : -1;
-          return key;
-        };
-        int next[2] = {-1, -1};
-        bool next_v = false;
-        int next_key = nblk > 0 ? rows_of(0, next, next_v) : 0;
-        for (int i = 0; i < 2 * nblk; ++i, ++pos) {
-          int row[2] = {next[0], next[1]};
-          const bool is_v = next_v;
-          const int key = next_key;
-          if (i + 1 < 2 * nblk) next_key = rows_of(i + 1, next, next_v);
-          bool bad = false;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (key + 32 * j < khi && (row[j] < 0 || row[j] >= a.kv_tokens)) {
-              bad = true;
-              row[j] = -1;
-            }
-          if (bad) atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-          const int st = pos % kStages;
-          ok = mbar_wait(&ctl.kv_empty[st], pos / kStages + 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const char* src = static_cast<const char*>(is_v ? a.v : a.k) + col;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int tok = __shfl_sync(0xffffffffu, row[j >> 4], (2 * j & 31) + sub);
-            cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes,
-                       src + (tok < 0 ? 0 : tok) * row_stride, tok < 0 ? 0 : 16);
+        if (nblk == 0) continue;
+        const int n = dual ? nblk : (nblk + 1 - s) >> 1;  // blocks of this stream
+        const int buf = dual ? s : qbuf;
+        for (int i = 0; i < 2; ++i)
+          if (dual || i == qbuf) {
+            ok = ok && mbar_wait(&ctl.q_full[i], q_uses[i], abort_flag);
+            ++q_uses[i];
+            if ((i != buf || n == 0) && lane == 0) mbar_arrive(&ctl.q_empty[i]);
           }
-          cp_async_arrive(&ctl.kv_full[st]);
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");   // nothing in flight when the CTA leaves
-    } else if (warp == kMmaWarp && lane == 0) {
-      // ---- products
-      uint32_t pos = 0, q_uses[2] = {0u, 0u}, p_uses[2] = {0u, 0u};
-      bool ok = true;
-      for (int it = 0; ok; ++it) {
-        const int slot = it & (kItems - 1);
-        if (!mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag)) break;
-        const Item& o = ctl.items[slot];
-        if (!o.valid) break;
-        const int dual = o.dual, nblk = o.nblk, qbuf = o.qbuf;
-        mbar_arrive(&ctl.item_empty[slot]);
-        const int n = dual ? 2 * nblk : nblk;            // steps; stream = step & 1
-        auto scores = [&](int i) {                       // S[stream] = Q K^T
-          const int s = i & 1, blk = dual ? i >> 1 : i, buf = dual ? s : qbuf;
-          if (dual ? i < 2 : i == 0) {
-            if (!mbar_wait(&ctl.q_full[buf], q_uses[buf], abort_flag)) return false;
-            ++q_uses[buf];
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint64_t dq = operand_desc(smem_u32(smem + kSmemQ + buf * kTileBytes), 16);
+        auto block = [&](int i) { return dual ? i : 2 * i + s; };
+        auto halves = [&](int i) { return keys - block(i) * kBlk > kHalf ? 2 : 1; };
+        auto scores = [&](int i, int h) {                // S = Q K^T of half h of the stream's i-th block
+          const uint32_t p = pos + ring_k(dual, block(i)), st = p % kStages;
+          if (h == 0) {
+            if (!have(p)) return false;
+            fence_async_smem();
           }
-          const uint32_t p = pos + ring_k(dual, blk), st = p % kStages;
-          if (!mbar_wait(&ctl.kv_full[st], p / kStages, abort_flag)) return false;
-          fence_async_smem();
           tc_fence_after();
-          const uint64_t dq = operand_desc(smem_u32(smem + kSmemQ + buf * kTileBytes), 16);
-          const uint64_t dk = operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes), 16);
+          const uint64_t dk =
+              operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes) + h * (kHalf * 128), 16);
+          const uint32_t b = t_qk++ & 1;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
-            mma_ss(tmem + s * 128, dq + off, dk + off, k > 0);
+            for (int k = 0; k < 8; ++k) {
+              const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
+              mma_ss(t_s + b * kHalf, dq + off, dk + off, k > 0);
+            }
+            mma_commit(&ctl.s_full[s][b]);
+            if (h + 1 == halves(i)) {
+              mma_commit(&ctl.kv_empty[st]);
+              if (i == n - 1) mma_commit(&ctl.q_empty[buf]);
+            }
           }
-          mma_commit(&ctl.s_full[s]);
-          if (!dual || s == 1) mma_commit(&ctl.kv_empty[st]);
-          if (dual ? blk == nblk - 1 : i == n - 1) mma_commit(&ctl.q_empty[buf]);
+          __syncwarp();
           return true;
         };
-        for (int i = 0; i < min(2, n) && ok; ++i) ok = scores(i);
+        // two steps of scores ahead of the weights
+        int qi = 0, qh = 0;
+        auto next_scores = [&]() {
+          if (qi >= n) return true;
+          const int i = qi, h = qh;
+          if (++qh == halves(i)) qh = 0, ++qi;
+          return scores(i, h);
+        };
+        ok = next_scores() && next_scores();
         for (int i = 0; i < n && ok; ++i) {
-          const int s = i & 1, blk = dual ? i >> 1 : i;
-          ok = mbar_wait(&ctl.p_full[s], p_uses[s], abort_flag);
-          if (!ok) break;
-          ++p_uses[s];
-          const uint32_t p = pos + ring_v(dual, blk, nblk), st = p % kStages;
-          ok = mbar_wait(&ctl.kv_full[st], p / kStages, abort_flag);
-          if (!ok) break;
-          fence_async_smem();
-          tc_fence_after();
-          const uint64_t dv = operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes), kHalfBytes);
+          const int nh = halves(i);
+          const uint32_t p = pos + ring_v(dual, block(i), nblk), st = p % kStages;
+          for (int h = 0; h < nh && ok; ++h) {
+            const uint32_t b = t_pv & 1;
+            const uint64_t dv =
+                operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes) + h * (kHalf * 128), kHalfBytes);
+            if (h == 0) {
+              ok = have(p);
+              if (!ok) break;
+            }
+            ok = mbar_wait(&ctl.p_full[s][b], t_pv >> 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++t_pv;
+            fence_async_smem();
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)                    // 16 keys each: two eight-row groups
-            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4),
-                   i >= 2 || k > 0);
-          if (!dual || s == 1) mma_commit(&ctl.kv_empty[st]);
-          if (i + 2 >= n) mma_commit(&ctl.o_full[s]);
-          if (i + 2 < n) ok = scores(i + 2);
+              for (int k = 0; k < 4; ++k)                // 16 keys each: two eight-row groups of V
+                mma_ts(t_o, t_s + b * kHalf + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4),
+                       i > 0 || h > 0 || k > 0);
+              mma_commit(&ctl.o_done[s][b]);
+              if (h + 1 == nh) mma_commit(&ctl.kv_empty[st]);
+            }
+            __syncwarp();
+            ok = next_scores();
+          }
         }
+        ok = ok && have(pos + 2 * nblk - 1);
         pos += 2 * nblk;
       }
     }
@@ -677,7 +799,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     const float scale = a.sm_scale * 1.4426950408889634f;
     const float slack = 8.f / scale;                     // scores may exceed the kept maximum by this
     char* const slots = static_cast<char*>(a.workspace) + kCutBytes;
-    uint32_t s_uses = 0, o_uses[2] = {0, 0}, j_uses = 0, pos = 0;
+    uint32_t t = 0, j_uses = 0, pos = 0;                 // t: steps of this stream so far
     bool ok = true;
     auto both_streams = [&]() {                          // barrier of the eight softmax warps, bounded
       __syncwarp();
@@ -693,76 +815,25 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       Item& o = ctl.items[islot];
       if (!o.valid) break;
       const int dual = o.dual, nblk = o.nblk, ntok = o.ntok;
-      const int t = (dual ? s * tile_tokens : 0) + r / G;
-      const bool live = r < tile_tokens * G && t < ntok;
+      const int token = (dual ? s * tile_tokens : 0) + r / G;
+      const bool live = r < tile_tokens * G && token < ntok;
       const bool any_live = __any_sync(0xffffffffu, live);
-      const int p = o.pos0 + t;
+      const int p = o.pos0 + token;
       // keys of this row; padding rows take all (they are computed and thrown away)
       const int key_lo = live && a.window >= 0 ? static_cast<int>(max(0ll, static_cast<long long>(p) + 1 - a.window)) : 0;
       const int key_hi = live ? p + 1 : INT_MAX;
       const int first = o.k0 + o.blk0 * kBlk;
       float m = -INFINITY, l = 0.f;
       const int step = dual ? 1 : 2, blk_first = dual ? 0 : s;
-      for (int blk = blk_first; blk < nblk; blk += step) {
-        ok = mbar_wait(&ctl.s_full[s], s_uses, abort_flag);
+      for (int blk = blk_first; blk < nblk && ok; blk += step) {
+       const int kb = first + blk * kBlk, nh = o.khi - kb > kHalf ? 2 : 1;
+       for (int h = 0; h < nh; ++h) {
+        const uint32_t b = t & 1, t_sb = t_s + b * kHalf;
+        ok = mbar_wait(&ctl.s_full[s][b], t >> 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        ++s_uses;
         tc_fence_after();
-        const int kb = first + blk * kBlk;
-        if (any_live) {
-          uint32_t u[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, u[c]);
-          tmem_ld_wait();
-          const int c_lo = key_lo - kb, c_hi = key_hi > kb + kBlk ? kBlk : key_hi - kb;   // columns in [c_lo, c_hi)
-          if (__any_sync(0xffffffffu, c_lo > 0 || c_hi < kBlk)) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c * 32 + i < c_lo || c * 32 + i >= c_hi) u[c][i] = 0xff800000u;
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[c][i]));
-          const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const bool grow = bm > m + slack || (m == -INFINITY && bm > m);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - bm) * scale);
-            if (grow) m = bm;
-            l *= f;
-            if (blk != blk_first) {                      // the product before this one has finished
-#pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                uint32_t w[32];
-                tmem_ld32(t_o + c * 32, w);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
-                tmem_st32(t_o + c * 32, w);
-              }
-            }
-          }
-          const float ms = m == -INFINITY ? 0.f : m * scale;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e0 = ex2(fmaf(__uint_as_float(u[c][2 * i]), scale, -ms));
-              const float e1 = ex2(fmaf(__uint_as_float(u[c][2 * i + 1]), scale, -ms));
-              sum[i & 3] += e0 + e1;
-              w[i] = pack_bf16(e0, e1);
-            }
-            tmem_st16(t_s + c * 16, w);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        }
-        if (partly_attended(o, a.window, kb)) {
+        if (h == 0 && partly_attended(o, a.window, kb)) {
           // A weight of zero does not silence an infinite or NaN value in the product.  Such values
           // of a block that some rows attend only in part are taken out here and put back, for the
           // rows that do attend them, when the unit ends.
@@ -791,28 +862,113 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
               }
           }
           fence_async_smem();
+          __syncwarp();                                  // the tensor-memory instructions want whole warps
+        }
+        if (!any_live) {                                 // rows that nobody reads: any weights will do
+          if (lane == 0) mbar_arrive(&ctl.p_full[s][b]);
+          __syncwarp();
+          ++t;
+          continue;
+        }
+        uint32_t u[2][32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) tmem_ld32(t_sb + c * 32, u[c]);
+        tmem_ld_wait();
+        loaded(u[0]);
+        loaded(u[1]);
+        const int ks = kb + h * kHalf;
+        const int c_lo = key_lo - ks, c_hi = key_hi > ks + kHalf ? kHalf : key_hi - ks;   // columns in [c_lo, c_hi)
+        if (__any_sync(0xffffffffu, c_lo > 0 || c_hi < kHalf)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i < c_lo || c * 32 + i >= c_hi) u[c][i] = 0xff800000u;
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t* x = &u[c >> 1][(c & 1) * 16];
+          mx[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+#pragma unroll
+          for (int i = 3; i < 15; i += 2) mx[c] = max3(mx[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        }
+        mx[0] = max3(mx[0], __uint_as_float(u[0][15]), __uint_as_float(u[0][31]));
+        mx[1] = max3(mx[1], __uint_as_float(u[1][15]), __uint_as_float(u[1][31]));
+        const float bm = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        const bool grow = bm > m + slack || (m == -INFINITY && bm > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - bm) * scale);
+          if (grow) m = bm;
+          l *= f;
+          if (blk != blk_first || h > 0) {
+            // the product of the step before has to be in
+            ok = mbar_wait(&ctl.o_done[s][b ^ 1], (t - 1) >> 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[32];
+              tmem_ld32(t_o + c * 32, w);
+              tmem_ld_wait();
+              loaded(w);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+              tmem_st32(t_o + c * 32, w);
+            }
+          }
+        }
+        // A logit of NaN or +inf makes the row NaN from here on (softmax of it is NaN).
+        if (!(bm < INFINITY)) m = __uint_as_float(0x7fc00000u);
+        const float ms = m == -INFINITY ? 0.f : m * scale;
+        const uint64_t scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float e0, e1;
+            unpair(fma2(pair(__uint_as_float(u[c][2 * i]), __uint_as_float(u[c][2 * i + 1])), scale2, ms2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            u[c][2 * i] = __float_as_uint(e0);
+            u[c][2 * i + 1] = __float_as_uint(e1);
+            w[i] = pack_bf16(e0, e1);
+          }
+          tmem_st16(t_sb + c * 16, w);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.p_full[s]);
+        if (lane == 0) mbar_arrive(&ctl.p_full[s][b]);
+        uint64_t sum[2] = {0ull, 0ull};                  // while the product runs
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sum[c] = add2(sum[c], pair(__uint_as_float(u[c][2 * i]), __uint_as_float(u[c][2 * i + 1])));
+        float l0, l1;
+        unpair(add2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
+        ++t;
+       }
       }
       if (!ok) break;
       pos += 2 * nblk;
       // ---- the unit's (part's) result.  Dual: a thread's own row.  Single: both streams hold a share
       // of every row; stream 0 finishes dims 0-63 and stream 1 dims 64-127.
-      const int phases[2] = {nblk > 0 ? 1 : 0, nblk > (dual ? 0 : 1) ? 1 : 0};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (phases[i] && (!dual || i == s)) ok = ok && mbar_wait(&ctl.o_full[i], o_uses[i], abort_flag);
-        o_uses[i] += phases[i];
+      if (blk_first < nblk) {
+        ok = mbar_wait(&ctl.o_done[s][(t - 1) & 1], (t - 1) >> 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
       }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
       float fa = 1.f, fb = 0.f;                          // what the accumulators are multiplied by
       if (!dual) {
         ctl.ml[s][r] = make_float2(m, l);
-        ok = both_streams();
+        tc_fence_before();
+        ok = both_streams();                             // the other stream's results are there too
         if (!ok) break;
         const float2 x = ctl.ml[0][r], y = ctl.ml[1][r];
         m = fmaxf(x.x, y.x);
@@ -826,7 +982,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       __threadfence_block();
       const bool refill = *reinterpret_cast<volatile unsigned*>(&o.nonfinite) != 0u;
       const bool cut = o.parts > 1;
-      const int64_t orow = static_cast<int64_t>(o.tok0 + t) * a.Hq + o.kh * G + r % G;
+      const int64_t orow = static_cast<int64_t>(o.tok0 + token) * a.Hq + o.kh * G + r % G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       float* const part = reinterpret_cast<float*>(slots + static_cast<int64_t>(o.slot) * kSlotBytes);
       const int prow = dual ? s * kRows + r : r;
@@ -835,10 +991,12 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
 #pragma unroll 1
         for (int c = dual ? 0 : 2 * s; c < (dual ? 4 : 2 * s + 2); ++c) {
           float v[32];
+          __syncwarp();
           if (nblk > 0) {
             uint32_t w[32];
             tmem_ld32(t_a + c * 32, w);
             tmem_ld_wait();
+            loaded(w);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]) * fa;
           } else {
@@ -849,6 +1007,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
             uint32_t w[32];
             tmem_ld32(t_a + 128 + c * 32, w);
             tmem_ld_wait();
+            loaded(w);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = fmaf(__uint_as_float(w[i]), fb, v[i]);
           }
@@ -879,10 +1038,10 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
               dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           } else if (live) {
-            float4* dst = reinterpret_cast<float4*>(part + prow * 128 + c * 32);
+            float4* dst = reinterpret_cast<float4*>(part) + c * 8 * kSlotRows + prow;   // four dims of all rows
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              dst[i * kSlotRows] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         }
       }
@@ -892,6 +1051,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         else if (a.lse)
           a.lse[orow] = l == 0.f ? -INFINITY : (m * scale + log2f(l)) * 0.6931471805599453f;
       }
+      __syncwarp();
       if (!dual) {
         tc_fence_before();
         ok = both_streams();                             // the accumulators and ctl.ml are free again
@@ -912,73 +1072,83 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
 }
 
 // ---------------------------------------------------------------------- units that were cut
-// Block (c, y) joins rows [16 y, 16 y + 16) of the unit that begins in part c.  A row's parts are
-// shared by as many of the eight warps as the rows leave free; four dims a lane.  The sums run in
-// an order that the parts alone decide.
+// Block (c, y) joins rows [16 y, 16 y + 16) of the unit that begins in part c.  A thread owns eight
+// dims of a row; where the rows leave threads free, the parts are shared among them too.  The sums
+// run in an order that the parts and rows alone decide.
 __global__ void __launch_bounds__(256)
 chunk_join_kernel(const MacB200ChunkArgs a) {
   const Cut cut = static_cast<const Cut*>(a.workspace)[blockIdx.x];
   const int G = a.Hq / a.Hkv, tile_tokens = kRows / G;
   const int row_first = blockIdx.y * kJoinRows, rows = min(cut.ntok * G - row_first, kJoinRows);
   if (cut.parts == 0 || rows <= 0) return;
-  __shared__ float4 acc_s[8][32];
-  __shared__ float l_s[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;   // warps of a row
+  __shared__ float4 acc_s[2][256];
+  __shared__ float l_s[256];
+  const int tid = threadIdx.x;
+  const int width = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;   // rows rounded up to a power of two
+  const int groups = 16 / width;                         // that share the parts
+  const int rr = tid % width, k = tid / width % 16, group = tid / (width * 16);
   const char* const slots = static_cast<const char*>(a.workspace) + kCutBytes;
   const float scale = a.sm_scale * 1.4426950408889634f;
-  const bool dual = cut.ntok > tile_tokens;
-  for (int rr = warp / share; rr < kJoinRows; rr += 8 / share) {
-    const bool live = rr < rows;
-    if (share == 1 && !live) break;
-    const int row = row_first + (live ? rr : 0);
-    const int token = row / G, g = row - token * G;
-    const int at = dual && token >= tile_tokens ? row - tile_tokens * G + kRows : row;
-    auto slot_of = [&](int i) {
-      return slots + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kSlotBytes;
-    };
-    float mx = -INFINITY;
-    for (int i = lane; i < cut.parts; i += 32)
-      mx = fmaxf(mx, reinterpret_cast<const float2*>(slot_of(i) + kSlotFloats * 4)[at].x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float ms = mx == -INFINITY ? 0.f : mx * scale;
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int row = row_first + min(rr, rows - 1);
+  const int token = row / G, g = row - token * G;
+  const bool second = cut.ntok > tile_tokens && token >= tile_tokens;
+  const int at = second ? row - tile_tokens * G + kRows : row;
+  auto slot_of = [&](int i) {
+    return slots + static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kSlotBytes;
+  };
+  float mx = -INFINITY;
 #pragma unroll 8
-    for (int i = warp % share; i < cut.parts; i += share) {
-      const char* sl = slot_of(i);
-      const float2 ml = reinterpret_cast<const float2*>(sl + kSlotFloats * 4)[at];
-      const float4 x = reinterpret_cast<const float4*>(sl)[at * 32 + lane];
-      if (ml.y != 0.f) {                                 // something attended in this part
-        const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x * scale - ms);   // NaN sums stay
-        l += ml.y * f;
-        acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
+  for (int i = group; i < cut.parts; i += groups)
+    mx = fmaxf(mx, reinterpret_cast<const float2*>(slot_of(i) + kSlotFloats * 4)[at].x);
+  if (groups > 1) {
+    l_s[tid] = mx;
+    __syncthreads();
+    for (int i = 0; i < groups; ++i) mx = fmaxf(mx, l_s[i * width * 16 + k * width + rr]);
+    __syncthreads();
+  }
+  const float ms = mx == -INFINITY ? 0.f : mx * scale;
+  float l = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+  for (int i = group; i < cut.parts; i += groups) {
+    const char* sl = slot_of(i);
+    const float2 ml = reinterpret_cast<const float2*>(sl + kSlotFloats * 4)[at];
+    const float4* x = reinterpret_cast<const float4*>(sl) + at;
+    const float4 x0 = x[k * kSlotRows], x1 = x[(k + 16) * kSlotRows];
+    if (ml.y != 0.f) {                                   // something attended in this part
+      const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x * scale - ms);   // NaN sums stay
+      l += ml.y * f;
+      acc[0].x += x0.x * f, acc[0].y += x0.y * f, acc[0].z += x0.z * f, acc[0].w += x0.w * f;
+      acc[1].x += x1.x * f, acc[1].y += x1.y * f, acc[1].z += x1.z * f, acc[1].w += x1.w * f;
+    }
+  }
+  if (groups > 1) {
+    acc_s[0][tid] = acc[0];
+    acc_s[1][tid] = acc[1];
+    l_s[tid] = l;
+    __syncthreads();
+    if (group != 0) return;
+    for (int i = 1; i < groups; ++i) {
+      const int t = i * width * 16 + tid;
+      l += l_s[t];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 x = acc_s[h][t];
+        acc[h].x += x.x, acc[h].y += x.y, acc[h].z += x.z, acc[h].w += x.w;
       }
     }
-    if (share > 1) {
-      acc_s[warp][lane] = acc;
-      if (lane == 0) l_s[warp] = l;
-      __syncthreads();
-      if (warp % share == 0)
-        for (int w = 1; w < share; ++w) {
-          const float4 x = acc_s[warp + w][lane];
-          l += l_s[warp + w];
-          acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
-        }
-      __syncthreads();
-    }
-    if (live && warp % share == 0) {
-      const float k = l == 0.f ? 0.f : 1.f / l;
-      const int64_t to = static_cast<int64_t>(cut.tok0 + token) * a.Hq + cut.kh * G + g;
-      uint2 w = make_uint2(0u, 0u);
-      if (l != 0.f) w = make_uint2(pack_bf16(acc.x * k, acc.y * k), pack_bf16(acc.z * k, acc.w * k));
-      *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + to * 256 + lane * 8) = w;
-      if (a.lse && lane == 0)
-        a.lse[to] = l == 0.f ? -INFINITY : (ms + log2f(l)) * 0.6931471805599453f;
-    }
-    if (share > 1) break;                                // 8 / share rows cover them all
   }
+  if (rr >= rows) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t to = static_cast<int64_t>(cut.tok0 + token) * a.Hq + cut.kh * G + g;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint2 w = make_uint2(0u, 0u);
+    if (l != 0.f)
+      w = make_uint2(pack_bf16(acc[h].x * inv, acc[h].y * inv), pack_bf16(acc[h].z * inv, acc[h].w * inv));
+    *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + to * 256 + (k + 16 * h) * 8) = w;
+  }
+  if (a.lse && k == 0) a.lse[to] = l == 0.f ? -INFINITY : (ms + log2f(l)) * 0.6931471805599453f;
 }
 
 // One warp per (row, query head); a lane holds dims [4l, 4l+4).
@@ -1080,7 +1250,7 @@ int prepare_kernel(int device) {
   if (device >= 0 && device < 64 && ready[device].load(std::memory_order_acquire)) return MAC_B200_OK;
   cudaFuncAttributes attr{};
   MAC_CUDA(cudaFuncGetAttributes(&attr, chunk_attention_kernel));
-  if (attr.numRegs * kThreads < 256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs)
+  if (attr.numRegs * kThreads < 256 * kSoftmaxRegs + 128 * (kControlRegs + kLoadRegs))
     return fail(MAC_B200_EUNSUPPORTED, "the chunk attention kernel was built with %d registers a thread",
                 attr.numRegs);
   MAC_CUDA(cudaFuncSetAttribute(chunk_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
