@@ -18,12 +18,12 @@
 // the parts, so the result does not depend on timing.
 //
 // Roles of a CTA (one per SM):
-//   warps 0-3 / 4-7  softmax streams 0 / 1, one thread per row: scores from tensor memory, running
+//   warps 8-15       softmax streams 0 and 1, a thread a row: scores from tensor memory, running
 //                    maximum and sum in fp32, bf16 weights back over the scores, results out
-//   warps 8, 9       issue the streams' products: S = Q K^T from shared memory, O += P V with P from
+//   warps 0, 1       issue the streams' products: S = Q K^T from shared memory, O += P V with P from
 //                    tensor memory and V from the rows as they lie in the pool (keys x dims)
-//   warps 12-15      fetch K/V rows by the page table into the swizzled operand layout (cp.async)
-//   warp 10          works out the units of this CTA's part, fetches the query tiles
+//   warps 4-7        fetch K/V rows by the page table into the swizzled operand layout (cp.async)
+//   warp 2           works out the units of this CTA's part, fetches the query tiles
 // The running maximum is kept until a row's scores exceed it by 2^8 in weight: the rescaling of O
 // is rare, and exact when it happens.  Weights are rounded to bf16 for the second product (the
 // operand type); the sum of weights is taken before that rounding, in fp32.
@@ -48,17 +48,17 @@ constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 bf16 in the 128-byte
 constexpr int kTileBytes = 2 * kHalfBytes;
 constexpr int kStages = 5;                 // K/V blocks in shared memory
 constexpr int kItems = 4;                  // units announced ahead
-constexpr int kSoftmaxWarps = 8;
-constexpr int kMmaWarp = 8, kPlanWarp = 10, kLoadWarp = 12, kLoadWarps = 4;
+// Warps by role.  The issuing warps come first: a scheduler prefers its older warps.
+constexpr int kMmaWarp = 0, kPlanWarp = 2, kLoadWarp = 4, kLoadWarps = 4, kSoftmaxWarp = 8, kSoftmaxWarps = 8;
 constexpr int kThreads = 512;
-// registers a thread after the warpgroups have traded theirs: 256 * 152 + 128 * 96 + 128 * 112 = 512 * 128
-constexpr int kSoftmaxRegs = 152, kControlRegs = 96, kLoadRegs = 112;
+// registers a thread after the warpgroups have traded theirs: 128 * 96 + 128 * 112 + 256 * 152 = 512 * 128
+constexpr int kLaunchRegs = 128, kControlRegs = 96, kLoadRegs = 112, kSoftmaxRegs = 152;
 constexpr int kUnitCells = 1;              // what a unit costs beside its blocks, in blocks
 constexpr int kMinCells = 3;               // least work worth a CTA of its own, where units are long
 constexpr int kJoinRows = 16;              // rows of a unit that a block of the second kernel joins
 constexpr int kTmemCols = 512;             // S0 S1 O0 O1; the weights lie over the scores
 constexpr int kRowWarps = 8;
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+constexpr long long kWaitLimitClocks = 4000000000ll;   // about two seconds
 
 // The workspace: a list of the units that were cut (entry c: the one that begins in CTA c's part
 // and ends behind it), then two slots a CTA for a part's unnormalised results, 256 rows each.
@@ -114,11 +114,6 @@ static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
@@ -140,27 +135,21 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits for the phase of `count` earlier phases.  False when the limit ran out here or in another
-// warp of the CTA: the caller leaves its loop.
-__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, unsigned* abort_flag) {
-  unsigned long long t0 = 0;                             // the clock is slow to read: not before it is needed
-  for (unsigned spins = 1;; ++spins) {
-    if (mbar_try(bar, parity)) return true;              // each try may itself block for a while
-    if ((spins & 63u) == 0u) {
-      if (*reinterpret_cast<volatile unsigned*>(abort_flag) != 0u) return false;
-      if (t0 == 0) t0 = now_ns();
-      if (now_ns() - t0 > kWaitLimitNs) {
-        *reinterpret_cast<volatile unsigned*>(abort_flag) = 1u;
-        atomicOr(&g_chunk_status, MAC_B200_STATUS_COPY_TIMEOUT);
-        return false;
-      }
-    }
-  }
-}
+// Waits for the phase of the given parity.  False when the limit ran out here or in another warp of
+// the CTA: the caller leaves its loop.  Short on purpose: it stands at two dozen places, and what
+// the warps of a scheduler execute in turn has to stay in its instruction cache.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned* abort_flag) {
   const uint32_t b = smem_u32(bar);
   if (mbar_try(b, parity & 1u)) return true;
-  return mbar_wait_slow(b, parity & 1u, abort_flag);
+  const long long t0 = clock64();
+  while (!mbar_try(b, parity & 1u)) {                    // each try may itself block for a while
+    if (*reinterpret_cast<volatile unsigned*>(abort_flag) != 0u) return false;
+    if (clock64() - t0 > kWaitLimitClocks) {
+      *reinterpret_cast<volatile unsigned*>(abort_flag) = MAC_B200_STATUS_COPY_TIMEOUT;   // reported at the end
+      return false;
+    }
+  }
+  return true;
 }
 
 __device__ __forceinline__ void tc_fence_before() {
@@ -382,9 +371,8 @@ __device__ __forceinline__ long long scan_cta(long long mine, long long& before,
   return total;
 }
 
-// The ring position of block `blk`'s K and V within a unit: K and V in turn when both streams use
-// each block; one K ahead when the streams alternate (K0 K1 V0 K2 V1 ...).
-__device__ __forceinline__ int ring_k(int dual, int blk) { return dual ? 2 * blk : (blk == 0 ? 0 : 2 * blk - 1); }
+// The ring holds K and V in turn when both streams use each block, and is one K ahead when the
+// streams alternate (K0 K1 V0 K2 V1 ...).  Where in a unit's positions block `blk`'s V is:
 __device__ __forceinline__ int ring_v(int dual, int blk, int nblk) {
   return dual ? 2 * blk + 1 : min(2 * blk + 2, 2 * nblk - 1);
 }
@@ -404,13 +392,6 @@ __device__ __forceinline__ void ring_at(int dual, int nblk, int i, int& blk, boo
     blk = (i - 2) >> 1;
     is_v = true;
   }
-}
-
-// Whether some row of the unit attends only a part of the keys of block [kb, kb + 128) that exist.
-__device__ __forceinline__ bool partly_attended(const Item& it, int window, int kb) {
-  const int last = it.pos0 + it.ntok - 1;
-  return min(kb + kBlk, it.khi) > it.pos0 + 1 ||
-         (window >= 0 && static_cast<long long>(kb) < static_cast<long long>(last) + 1 - window);
 }
 
 __device__ __forceinline__ const void* v_row(const MacB200ChunkArgs& a, const Item& it, int key) {
@@ -479,7 +460,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       mbar_init(&ctl.q_empty[i], 2);
       for (int h = 0; h < 2; ++h) {
         mbar_init(&ctl.s_full[i][h], 1);
-        mbar_init(&ctl.p_full[i][h], 4);
+        mbar_init(&ctl.p_full[i][h], kSoftmaxWarps / 2);
         mbar_init(&ctl.o_done[i][h], 1);
       }
     }
@@ -503,7 +484,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(ctl.tmem)));
   unsigned* const abort_flag = &ctl.abort;
 
-  if (warp >= kLoadWarp) {
+  if (warp >= kLoadWarp && warp < kSoftmaxWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     // ---- K/V rows by the page table: sixteen lanes fetch a row, a warp 32 of a block's 128
     const int part = (warp - kLoadWarp) * 32;
@@ -516,7 +497,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
               (((chunk & 7) ^ (row & 7)) << 4);
     }
-    uint32_t pos = 0;
+    uint32_t st = 0, phase = 1;                          // of the ring position to fill next
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const int slot = it & (kItems - 1);
@@ -547,13 +528,12 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         return e;
       };
       Entry next = entry_of(0), after = entry_of(1);
-      for (int i = 0; i < 2 * nblk; ++i, ++pos) {
+      for (int i = 0; i < 2 * nblk; ++i) {
         const Entry e = next;
         next = after;
         after = entry_of(i + 2);
         const bool is_v = e.is_v;
-        const int st = pos % kStages;
-        ok = mbar_wait(&ctl.kv_empty[st], pos / kStages + 1, abort_flag);
+        ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const char* src = static_cast<const char*>(is_v ? a.v : a.k) + col;
@@ -571,10 +551,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
                      src + (tok < 0 ? 0 : tok) * row_stride, tok < 0 ? 0 : 16);
         }
         cp_async_arrive(&ctl.kv_full[st]);
+        if (++st == kStages) st = 0, phase ^= 1u;
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");   // nothing in flight when the CTA leaves
-  } else if (warp >= kSoftmaxWarps) {
+  } else if (warp < kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
 
     if (warp == kPlanWarp && lane == 0) {
@@ -665,9 +646,9 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       // a query tile still on its way when the CTA gives up must land before the CTA leaves
       if (*reinterpret_cast<volatile unsigned*>(abort_flag) != 0u)
         for (int i = 0; i < 2; ++i) {
-          const unsigned long long t0 = now_ns();
+          const long long t0 = clock64();
           while (q_uses[i] > 0 && !mbar_try(smem_u32(&ctl.q_full[i]), (q_uses[i] - 1) & 1u) &&
-                 now_ns() - t0 < kWaitLimitNs) {}
+                 clock64() - t0 < kWaitLimitClocks) {}
         }
     } else if (warp < kMmaWarp + 2) {
       // ---- the products of stream `warp - kMmaWarp`.  The whole warp walks through the steps and one
@@ -676,27 +657,15 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       // warp a stream: neither waits for the other's softmax.
       const int s = warp - kMmaWarp;
       const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
-      uint32_t pos = 0, seen = 0, q_uses[2] = {0u, 0u};
-      uint32_t t_qk = 0, t_pv = 0;                       // steps of 64 keys issued so far
+      // What one warp computes between two products is latency on the tensor cores' path: stages and
+      // phases are counted along, not divided out of positions, and descriptors are sums.
+      uint32_t q_phase[2] = {0u, 0u}, t = 0;             // t: steps of 64 keys so far
+      uint32_t st = 0, phase = 0;                        // of the ring position to wait for next
+      const uint64_t desc_q = operand_desc(smem_u32(smem + kSmemQ), 16);
+      const uint64_t desc_k = operand_desc(smem_u32(smem + kSmemKv), 16);
+      const uint64_t desc_v = operand_desc(smem_u32(smem + kSmemKv), kHalfBytes);
+      constexpr uint64_t kDescTile = kTileBytes >> 4, kDescHalf = (kHalf * 128) >> 4;
       bool ok = true;
-      int dual = 0, nblk = 0;
-      // A barrier tells its phases apart by one bit, so no phase may pass a waiter by: both streams'
-      // warps wait for every ring position in order, and each gives every position back -- with its
-      // last product on it, or at once when the block is the other stream's.  The same for query
-      // tiles.
-      auto have = [&](uint32_t p) {
-        bool good = true;
-        for (; good && seen <= p; ++seen) {
-          good = mbar_wait(&ctl.kv_full[seen % kStages], seen / kStages, abort_flag);
-          if (!dual) {
-            int blk;
-            bool is_v;
-            ring_at(0, nblk, static_cast<int>(seen - pos), blk, is_v);
-            if ((blk & 1) != s && lane == 0) mbar_arrive(&ctl.kv_empty[seen % kStages]);
-          }
-        }
-        return __all_sync(0xffffffffu, good) != 0;
-      };
       for (int it = 0; ok; ++it) {
         const int slot = it & (kItems - 1);
         ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
@@ -704,96 +673,105 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         if (!ok) break;
         const Item& o = ctl.items[slot];
         if (!uniform(o.valid)) break;
-        dual = uniform(o.dual);
-        nblk = uniform(o.nblk);
-        const int qbuf = uniform(o.qbuf), keys = uniform(o.khi - o.k0 - o.blk0 * kBlk);
+        const int dual = uniform(o.dual), nblk = uniform(o.nblk), qbuf = uniform(o.qbuf);
+        const int keys = uniform(o.khi - o.k0 - o.blk0 * kBlk);
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
         if (nblk == 0) continue;
         const int n = dual ? nblk : (nblk + 1 - s) >> 1;  // blocks of this stream
         const int buf = dual ? s : qbuf;
+        // A barrier tells its phases apart by one bit, so no phase may pass a waiter by: both streams'
+        // warps wait for every ring position in order, and each gives every position back -- with its
+        // last product on it, or at once when the block is the other stream's.  The same for query
+        // tiles.
         for (int i = 0; i < 2; ++i)
           if (dual || i == qbuf) {
-            ok = ok && mbar_wait(&ctl.q_full[i], q_uses[i], abort_flag);
-            ++q_uses[i];
+            ok = ok && mbar_wait(&ctl.q_full[i], q_phase[i], abort_flag);
+            q_phase[i] ^= 1u;
             if ((i != buf || n == 0) && lane == 0) mbar_arrive(&ctl.q_empty[i]);
           }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint64_t dq = operand_desc(smem_u32(smem + kSmemQ + buf * kTileBytes), 16);
-        auto block = [&](int i) { return dual ? i : 2 * i + s; };
-        auto halves = [&](int i) { return keys - block(i) * kBlk > kHalf ? 2 : 1; };
-        auto scores = [&](int i, int h) {                // S = Q K^T of half h of the stream's i-th block
-          const uint32_t p = pos + ring_k(dual, block(i)), st = p % kStages;
-          if (h == 0) {
-            if (!have(p)) return false;
-            fence_async_smem();
+        int at = 0;                                      // the next position within the unit
+        // waits for the stream's next own position; its stage, or -1
+        auto next_stage = [&]() {
+          while (ok) {
+            ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
+            bool mine = true;
+            if (!dual) {
+              int blk;
+              bool is_v;
+              ring_at(0, nblk, at, blk, is_v);
+              mine = (blk & 1) == s;
+              if (!mine && lane == 0) mbar_arrive(&ctl.kv_empty[st]);
+            }
+            const int found = static_cast<int>(st);
+            ++at;
+            if (++st == kStages) st = 0, phase ^= 1u;
+            if (mine) return found;
           }
-          tc_fence_after();
-          const uint64_t dk =
-              operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes) + h * (kHalf * 128), 16);
-          const uint32_t b = t_qk++ & 1;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
-              mma_ss(t_s + b * kHalf, dq + off, dk + off, k > 0);
-            }
-            mma_commit(&ctl.s_full[s][b]);
-            if (h + 1 == halves(i)) {
-              mma_commit(&ctl.kv_empty[st]);
-              if (i == n - 1) mma_commit(&ctl.q_empty[buf]);
-            }
-          }
-          __syncwarp();
-          return true;
+          return -1;
         };
-        // two steps of scores ahead of the weights
-        int qi = 0, qh = 0;
-        auto next_scores = [&]() {
-          if (qi >= n) return true;
-          const int i = qi, h = qh;
-          if (++qh == halves(i)) qh = 0, ++qi;
-          return scores(i, h);
-        };
-        ok = next_scores() && next_scores();
-        for (int i = 0; i < n && ok; ++i) {
-          const int nh = halves(i);
-          const uint32_t p = pos + ring_v(dual, block(i), nblk), st = p % kStages;
-          for (int h = 0; h < nh && ok; ++h) {
-            const uint32_t b = t_pv & 1;
-            const uint64_t dv =
-                operand_desc(smem_u32(smem + kSmemKv + st * kTileBytes) + h * (kHalf * 128), kHalfBytes);
-            if (h == 0) {
-              ok = have(p);
-              if (!ok) break;
-            }
-            ok = mbar_wait(&ctl.p_full[s][b], t_pv >> 1, abort_flag);
+        const uint64_t dq = desc_q + buf * kDescTile;
+        // The last block may hold one half only.  Scores run two steps ahead of the weights: step t
+        // takes score buffer t & 1, and its weights lie where its scores were.
+        const int steps = 2 * n - (n > 0 && keys - (dual ? n - 1 : 2 * (n - 1) + s) * kBlk <= kHalf ? 1 : 0);
+        int st_k = 0, st_v = 0;
+        for (int i = 0; i < (steps > 0 ? steps + 2 : 0); ++i) {
+          const int h = i & 1;
+          if (i >= 2) {                                  // O += P V of step i - 2
+            const uint32_t b = t & 1;
+            if (h == 0) st_v = next_stage();
+            ok = ok && mbar_wait(&ctl.p_full[s][b], t >> 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            ++t_pv;
+            ++t;
             fence_async_smem();
             tc_fence_after();
+            const uint64_t dv = desc_v + uniform(st_v) * kDescTile + h * kDescHalf;
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)                // 16 keys each: two eight-row groups of V
-                mma_ts(t_o, t_s + b * kHalf + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4),
-                       i > 0 || h > 0 || k > 0);
+                mma_ts(t_o, t_s + b * kHalf + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4), i > 2 || k > 0);
               mma_commit(&ctl.o_done[s][b]);
-              if (h + 1 == nh) mma_commit(&ctl.kv_empty[st]);
+              if (h == 1 || i == steps + 1) mma_commit(&ctl.kv_empty[st_v]);
             }
             __syncwarp();
-            ok = next_scores();
+          }
+          if (i < steps) {                               // S = Q K^T of step i, into the buffer just emptied
+            const uint32_t b = (i < 2 ? t + i : t - 1) & 1;
+            if (h == 0) {
+              st_k = next_stage();
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              fence_async_smem();
+            }
+            tc_fence_after();
+            const uint64_t dk = desc_k + uniform(st_k) * kDescTile + h * kDescHalf;
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
+                mma_ss(t_s + b * kHalf, dq + off, dk + off, k > 0);
+              }
+              mma_commit(&ctl.s_full[s][b]);
+              if (h == 1 || i == steps - 1) mma_commit(&ctl.kv_empty[st_k]);
+              if (i == steps - 1) mma_commit(&ctl.q_empty[buf]);
+            }
+            __syncwarp();
           }
         }
-        ok = ok && have(pos + 2 * nblk - 1);
-        pos += 2 * nblk;
+        while (ok && at < 2 * nblk) {                    // the other stream's last positions
+          ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
+          if (lane == 0) mbar_arrive(&ctl.kv_empty[st]);
+          ++at;
+          if (++st == kStages) st = 0, phase ^= 1u;
+        }
+        ok = __all_sync(0xffffffffu, ok);
       }
     }
   } else {
     // ---- softmax: this thread's row of its stream
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int s = warp >> 2, r = tid & 127;
+    const int s = (warp - kSoftmaxWarp) >> 2, r = tid & 127;
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + s * 128 + t_lane, t_o = tmem + 256 + s * 128 + t_lane;
     const float scale = a.sm_scale * 1.4426950408889634f;
@@ -823,17 +801,19 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       const int key_lo = live && a.window >= 0 ? static_cast<int>(max(0ll, static_cast<long long>(p) + 1 - a.window)) : 0;
       const int key_hi = live ? p + 1 : INT_MAX;
       const int first = o.k0 + o.blk0 * kBlk;
+      // keys that every row of the warp attends: [warp_lo, warp_hi); steps inside need no mask
+      const int warp_lo = __reduce_max_sync(0xffffffffu, key_lo), warp_hi = __reduce_min_sync(0xffffffffu, key_hi);
+      // and that every row of the unit does; blocks inside need no look at their values
+      const int unit_lo = a.window >= 0 ? o.pos0 + ntok - a.window : 0, unit_hi = o.pos0 + 1, khi = o.khi;
       float m = -INFINITY, l = 0.f;
       const int step = dual ? 1 : 2, blk_first = dual ? 0 : s;
       for (int blk = blk_first; blk < nblk && ok; blk += step) {
-       const int kb = first + blk * kBlk, nh = o.khi - kb > kHalf ? 2 : 1;
+       const int kb = first + blk * kBlk, nh = khi - kb > kHalf ? 2 : 1;
        for (int h = 0; h < nh; ++h) {
         const uint32_t b = t & 1, t_sb = t_s + b * kHalf;
         ok = mbar_wait(&ctl.s_full[s][b], t >> 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         tc_fence_after();
-        if (h == 0 && partly_attended(o, a.window, kb)) {
+        if (h == 0 && (min(kb + kBlk, khi) > unit_hi || kb < unit_lo)) {
           // A weight of zero does not silence an infinite or NaN value in the product.  Such values
           // of a block that some rows attend only in part are taken out here and put back, for the
           // rows that do attend them, when the unit ends.
@@ -878,7 +858,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         loaded(u[1]);
         const int ks = kb + h * kHalf;
         const int c_lo = key_lo - ks, c_hi = key_hi > ks + kHalf ? kHalf : key_hi - ks;   // columns in [c_lo, c_hi)
-        if (__any_sync(0xffffffffu, c_lo > 0 || c_hi < kHalf)) {
+        if (ks < warp_lo || ks + kHalf > warp_hi) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -897,7 +877,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         mx[1] = max3(mx[1], __uint_as_float(u[1][15]), __uint_as_float(u[1][31]));
         const float bm = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
         const bool grow = bm > m + slack || (m == -INFINITY && bm > m);
-        if (__any_sync(0xffffffffu, grow)) {
+        if (__any_sync(0xffffffffu, grow || !ok)) {
+          if (!__all_sync(0xffffffffu, ok)) {            // the wait for the scores gave up
+            ok = false;
+            break;
+          }
           const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - bm) * scale);
           if (grow) m = bm;
           l *= f;
@@ -1014,7 +998,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           if (refill && live) {
             for (int blk = 0; blk < nblk; ++blk) {
               const int kb = first + blk * kBlk;
-              if (!partly_attended(o, a.window, kb)) continue;
+              if (min(kb + kBlk, khi) <= unit_hi && kb >= unit_lo) continue;
               for (int key = max(kb, key_lo); key < min(kb + kBlk, key_hi); ++key) {
                 const uint32_t* x = static_cast<const uint32_t*>(v_row(a, o, key));
                 if (x == nullptr) continue;
@@ -1065,6 +1049,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && ctl.abort != 0u) atomicOr(&g_chunk_status, ctl.abort);
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
@@ -1250,7 +1235,7 @@ int prepare_kernel(int device) {
   if (device >= 0 && device < 64 && ready[device].load(std::memory_order_acquire)) return MAC_B200_OK;
   cudaFuncAttributes attr{};
   MAC_CUDA(cudaFuncGetAttributes(&attr, chunk_attention_kernel));
-  if (attr.numRegs * kThreads < 256 * kSoftmaxRegs + 128 * (kControlRegs + kLoadRegs))
+  if (attr.numRegs < kLaunchRegs)
     return fail(MAC_B200_EUNSUPPORTED, "the chunk attention kernel was built with %d registers a thread",
                 attr.numRegs);
   MAC_CUDA(cudaFuncSetAttribute(chunk_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
@@ -1260,7 +1245,8 @@ int prepare_kernel(int device) {
 
 int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
   MAC_REQUIRE(args != nullptr, "chunk args must not be null");
-  const MacB200ChunkArgs& a = *args;
+  MacB200ChunkArgs a = *args;
+  if (a.window >= (1 << 30)) a.window = -1;              // longer than any cache
   MAC_REQUIRE(a.D == 128, "chunk attention needs D=128");
   MAC_REQUIRE(a.Hq > 0 && a.Hkv > 0 && a.Hq % a.Hkv == 0 && a.Hq / a.Hkv <= 16,
               "Hq must be Hkv times 1..16");
