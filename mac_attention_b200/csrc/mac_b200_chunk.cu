@@ -18,11 +18,12 @@
 // the parts, so the result does not depend on timing.
 //
 // Roles of a CTA (one per SM):
-//   warps 8-15       softmax streams 0 and 1, a thread a row: scores from tensor memory, running
+//   the last eight   softmax streams 0 and 1, a thread a row: scores from tensor memory, running
 //                    maximum and sum in fp32, bf16 weights back over the scores, results out
 //   warps 0, 1       issue the streams' products: S = Q K^T from shared memory, O += P V with P from
 //                    tensor memory and V from the rows as they lie in the pool (keys x dims)
-//   warps 4-7        fetch K/V rows by the page table into the swizzled operand layout (cp.async)
+//   warps 4-7 (-11)  fetch K/V rows by the page table into the swizzled operand layout (cp.async; the
+//                    8-bit pool's rows by way of a raw buffer, widened to bf16)
 //   warp 2           works out the units of this CTA's part, fetches the query tiles
 // The running maximum is kept until a row's scores exceed it by 2^8 in weight: the rescaling of O
 // is rare, and exact when it happens.  Weights are rounded to bf16 for the second product (the
@@ -46,18 +47,14 @@ constexpr int kRows = 128;                 // rows of a tile
 constexpr int kHalf = 64;                  // keys of a step: what a stream takes from scores to weights at once
 constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 bf16 in the 128-byte-swizzled layout
 constexpr int kTileBytes = 2 * kHalfBytes;
-constexpr int kStages = 5;                 // K/V blocks in shared memory
+constexpr int kMaxStages = 5;              // K/V blocks in shared memory
 constexpr int kItems = 4;                  // units announced ahead
 // Warps by role.  The issuing warps come first: a scheduler prefers its older warps.
-constexpr int kMmaWarp = 0, kPlanWarp = 2, kLoadWarp = 4, kLoadWarps = 4, kSoftmaxWarp = 8, kSoftmaxWarps = 8;
-constexpr int kThreads = 512;
-// registers a thread after the warpgroups have traded theirs: 128 * 96 + 128 * 112 + 256 * 152 = 512 * 128
-constexpr int kLaunchRegs = 128, kControlRegs = 96, kLoadRegs = 112, kSoftmaxRegs = 152;
+constexpr int kMmaWarp = 0, kPlanWarp = 2, kLoadWarp = 4, kSoftmaxWarps = 8;
 constexpr int kUnitCells = 1;              // what a unit costs beside its blocks, in blocks
 constexpr int kMinCells = 3;               // least work worth a CTA of its own, where units are long
 constexpr int kJoinRows = 16;              // rows of a unit that a block of the second kernel joins
 constexpr int kTmemCols = 512;             // S0 S1 O0 O1; the weights lie over the scores
-constexpr int kRowWarps = 8;
 constexpr long long kWaitLimitClocks = 4000000000ll;   // about two seconds
 
 // The workspace: a list of the units that were cut (entry c: the one that begins in CTA c's part
@@ -93,11 +90,11 @@ struct Item {
 };
 
 struct Control {
-  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
   uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2];
   uint64_t item_full[kItems], item_empty[kItems], join;
   Item items[kItems];
-  long long scan[kThreads / 32];
+  long long scan[20];      // a word a warp
   long long start_pos;     // where request start_b begins on the line
   int start_b;
   uint32_t tmem;
@@ -105,11 +102,29 @@ struct Control {
   float2 ml[2][kRows];     // a single unit's maxima and sums, by stream
 };
 
+// Shared memory: two query tiles, the ring of K/V blocks, for the 8-bit pool the raw rows on their
+// way (each thread of the loading warps reads back what it fetched itself), the control words.
+// Registers a thread after the warpgroups have traded theirs:
+//   bf16: 128 * 64 + 128 * 160 + 256 * 144 = 512 * 128,  e4m3: 128 * 64 + 256 * 72 + 256 * 136 = 640 * 96
 constexpr int kSmemQ = 0;
 constexpr int kSmemKv = 2 * kTileBytes;
-constexpr int kSmemControl = kSmemKv + kStages * kTileBytes;
-constexpr int kSmemBytes = kSmemControl + static_cast<int>(sizeof(Control));
-static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
+constexpr int kRawSlots = 3;
+template <bool kE4m3>
+struct Layout {
+  static constexpr int kLoadWarps = kE4m3 ? 8 : 4;
+  static constexpr int kSoftmaxWarp = kLoadWarp + kLoadWarps;
+  static constexpr int kThreads = 32 * (kSoftmaxWarp + kSoftmaxWarps);
+  static constexpr int kLaunchRegs = kE4m3 ? 96 : 128, kControlRegs = 64;
+  static constexpr int kLoadRegs = kE4m3 ? 72 : 160, kSoftmaxRegs = kE4m3 ? 136 : 144;
+  static constexpr int kWarpRows = kBlk / kLoadWarps;    // rows of a block that a loading warp fetches
+  static constexpr int kStages = kE4m3 ? 3 : kMaxStages;
+  static constexpr int kRawRows = kWarpRows * 128;       // of a warp and a ring position
+  static constexpr int kRawBytes = kRawRows + kWarpRows * 4;   // and the words that hold the exponents
+  static constexpr int kRaw = kSmemKv + kStages * kTileBytes;
+  static constexpr int kControl = kRaw + (kE4m3 ? kRawSlots * kLoadWarps * kRawBytes : 0);
+  static constexpr int kBytes = kControl + static_cast<int>(sizeof(Control));
+};
+static_assert(Layout<false>::kBytes <= 232448 && Layout<true>::kBytes <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -273,6 +288,9 @@ __device__ __forceinline__ int load_early(const int32_t* p) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 // arrives on `bar` once this thread's copies so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -350,6 +368,7 @@ __device__ __forceinline__ long long head_cells(const Request& r, int window, in
 }
 
 // Sum over the CTA of `mine`; `before` gets what the threads before this one hold.
+template <int kThreads>
 __device__ __forceinline__ long long scan_cta(long long mine, long long& before, long long* warps) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long x = mine;
@@ -394,17 +413,62 @@ __device__ __forceinline__ void ring_at(int dual, int nblk, int i, int& blk, boo
   }
 }
 
-__device__ __forceinline__ const void* v_row(const MacB200ChunkArgs& a, const Item& it, int key) {
+// Dims [d, d + 2) of the value of key `key`; zeros where the page table leads outside the pool.
+template <bool kE4m3>
+__device__ __forceinline__ float2 value_pair(const MacB200ChunkArgs& a, const Item& it, int key, int d) {
   const int tok = a.req_to_token[static_cast<int64_t>(it.req) * a.req_to_token_stride + key];
-  if (tok < 0 || tok >= a.kv_tokens) return nullptr;
-  return static_cast<const char*>(a.v) + (static_cast<int64_t>(tok) * a.Hkv + it.kh) * 256;
+  if (tok < 0 || tok >= a.kv_tokens) return make_float2(0.f, 0.f);
+  const int64_t row = static_cast<int64_t>(tok) * a.Hkv + it.kh;
+  if (!kE4m3) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v) + row * 256 + d * 2);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  const float2 x = kv8_unpack2(*reinterpret_cast<const uint16_t*>(static_cast<const char*>(a.v) + row * 128 + d));
+  const uint32_t w = pack_bf16(x.x * kv8_scale(a.v_exp[row]), x.y * kv8_scale(a.v_exp[row]));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// ------------------------------------------------------------------------------------ the kernel
-__global__ void __launch_bounds__(kThreads, 1)
+// ------------------------------------------------------------------- rows of the 8-bit pool
+__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
+  __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// Sixteen codes of a row to bf16 (eight words), without a branch, and whether that was not enough.
+// An e4m3 number's exponent and mantissa bits, moved to where bf16 has its own, read as the number
+// times 2^-120 (the difference of the biases), subnormal codes included; one factor puts the row's
+// scale on, exactly.  Not enough: codes of NaN, and rows whose factor would overflow (past 448 * 2^7).
+__device__ __forceinline__ bool widen16(const uint4& c, int e, uint32_t (&w)[8]) {
+  const uint32_t code[4] = {c.x, c.y, c.z, c.w};
+  const uint32_t f = e == kKv8NanExp ? 0x7fc0u : static_cast<uint32_t>(min(e, 134) + 120) << 7;
+  const uint32_t f2 = f | (f << 16);
+  uint32_t odd = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = __byte_perm(code[i], 0u, 0x1404), y = __byte_perm(code[i], 0u, 0x3424);
+    w[2 * i] = mul_bf16(((x >> 4) & 0x07f007f0u) | (x & 0x80008000u), f2);
+    w[2 * i + 1] = mul_bf16(((y >> 4) & 0x07f007f0u) | (y & 0x80008000u), f2);
+    odd |= (code[i] & 0x7f7f7f7fu) + 0x01010101u;
+  }
+  return (odd & 0x80808080u) != 0u || (e > 134 && e != kKv8NanExp);
+}
+__device__ __forceinline__ void widen16_seldom(const uint4& c, int e, uint32_t (&w)[8]) {
+  const uint32_t code[4] = {c.x, c.y, c.z, c.w};
+  const float s = kv8_scale(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 x = kv8_unpack2(code[i >> 1] >> ((i & 1) * 16));
+    w[i] = pack_bf16(x.x * s, x.y * s);
+  }
+}
+
+template <bool kE4m3>
+__global__ void __launch_bounds__(Layout<kE4m3>::kThreads, 1)
 chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtensorMap q_map) {
   extern __shared__ __align__(1024) uint8_t smem[];      // the swizzle repeats every 1024 bytes
-  Control& ctl = *reinterpret_cast<Control*>(smem + kSmemControl);
+  using L = Layout<kE4m3>;
+  constexpr int kStages = L::kStages, kThreads = L::kThreads, kLoadWarps = L::kLoadWarps;
+  constexpr int kSoftmaxWarp = L::kSoftmaxWarp;
+  Control& ctl = *reinterpret_cast<Control*>(smem + Layout<kE4m3>::kControl);
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int G = a.Hq / a.Hkv;
   const int tile_tokens = kRows / G;
@@ -417,7 +481,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   for (int b = b0; b < b1; ++b)
     mine += a.Hkv * static_cast<long long>((load_request(a, b, blockIdx.x == 0).n + tile_tokens - 1) / tile_tokens);
   // pairs of tiles once there are enough of them for every CTA
-  const int span = scan_cta(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
+  const int span = scan_cta<kThreads>(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
   long long units = 0;
   mine = 0;
   for (int b = b0; b < b1; ++b) {
@@ -426,8 +490,8 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     units += a.Hkv * static_cast<long long>((r.n + span - 1) / span);
   }
   long long unused;
-  units = scan_cta(units, unused, ctl.scan);
-  const long long total = scan_cta(mine, before, ctl.scan);
+  units = scan_cta<kThreads>(units, unused, ctl.scan);
+  const long long total = scan_cta<kThreads>(mine, before, ctl.scan);
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(units, total / kMinCells)));
   if (tid == 0) cuts[blockIdx.x].parts = 0;
   if (static_cast<int>(blockIdx.x) >= ctas) return;
@@ -452,7 +516,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   // ---- barriers, tensor memory
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&ctl.kv_full[i], kLoadWarps * 32);
+      mbar_init(&ctl.kv_full[i], kE4m3 ? kLoadWarps : kLoadWarps * 32);
       mbar_init(&ctl.kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
@@ -485,65 +549,85 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   unsigned* const abort_flag = &ctl.abort;
 
   if (warp >= kLoadWarp && warp < kSoftmaxWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
-    // ---- K/V rows by the page table: sixteen lanes fetch a row, a warp 32 of a block's 128
-    const int part = (warp - kLoadWarp) * 32;
-    const int sub = lane >> 4, chunk = lane & 15;
-    const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 256;
-    uint32_t to[4];                                    // where this lane's chunk goes in rows 2i + sub
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = part + 2 * i + sub;
-      to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
-              (((chunk & 7) ^ (row & 7)) << 4);
-    }
+    if constexpr (kE4m3)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kLoadRegs));
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kLoadRegs));
+    const int part = (warp - kLoadWarp) * L::kWarpRows;  // this warp's rows of a block
+    // What the table says of row `lane` of this warp's part, and where its rows lie.  Entries are
+    // asked for ahead and looked at when they are needed.
+    struct Entry {
+      bool valid, exists, is_v;
+      int row, kh;
+    };
+    // The ring positions of this CTA's units, one after the other.  An entry that is not valid: there
+    // are no more (`more` is false), or the next unit is not announced yet.  A warp may wait for that
+    // only when it holds no position back: the announcement may wait for units that need it.
+    int it = 0, at = 0, dual = 0, nblk = 0, khi = 0, first = 0, kh = 0;
+    const int32_t* table = nullptr;
+    bool ok = true, more = true;
+    auto next_entry = [&](bool wait) {
+      Entry e{false, false, false, -1, 0};
+      while (more && at >= 2 * nblk) {                   // on to the next unit
+        const int slot = it & (kItems - 1);
+        if (wait)
+          ok = ok && mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
+        else if (!__all_sync(0xffffffffu, mbar_try(smem_u32(&ctl.item_full[slot]), (it / kItems) & 1)))
+          return e;
+        ok = __all_sync(0xffffffffu, ok);
+        const Item& o = ctl.items[slot];
+        more = ok && o.valid;
+        if (!more) break;
+        dual = o.dual;
+        nblk = o.nblk;
+        khi = o.khi;
+        first = o.k0 + o.blk0 * kBlk;
+        kh = o.kh;
+        table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
+        at = 0;
+        ++it;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
+      }
+      if (!more) return e;
+      int blk;
+      ring_at(dual, nblk, at++, blk, e.is_v);
+      const int key = first + blk * kBlk + part + lane;
+      e.valid = true;
+      e.exists = lane < L::kWarpRows && key < khi;
+      e.kh = kh;
+      if (e.exists) e.row = load_early(table + key);
+      return e;
+    };
+    // the pool row of an entry; -1: no key, or one outside the pool (reported): arrives as zeros
+    auto row_of = [&](const Entry& e) {
+      if (!e.exists) return -1;
+      if (e.row >= 0 && e.row < a.kv_tokens) return e.row;
+      atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+      return -1;
+    };
     uint32_t st = 0, phase = 1;                          // of the ring position to fill next
-    bool ok = true;
-    for (int it = 0; ok; ++it) {
-      const int slot = it & (kItems - 1);
-      ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const Item& o = ctl.items[slot];
-      if (!o.valid) break;
-      const int dual = o.dual, nblk = o.nblk, khi = o.khi;
-      const int first = o.k0 + o.blk0 * kBlk;
-      const int64_t col = o.kh * 256 + chunk * 16;
-      const int32_t* table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
-      // Key `lane` of this warp's part of ring position i: the key, and what the table says of it.
-      // Table entries are asked for two positions ahead and looked at when they are needed.
-      struct Entry {
-        int key, row;
-        bool is_v;
-      };
-      auto entry_of = [&](int i) {
-        Entry e{khi, 0, false};
-        if (i >= 2 * nblk) return e;
-        int blk;
-        ring_at(dual, nblk, i, blk, e.is_v);
-        e.key = first + blk * kBlk + part + lane;
-        if (e.key < khi) e.row = load_early(table + e.key);
-        return e;
-      };
-      Entry next = entry_of(0), after = entry_of(1);
-      for (int i = 0; i < 2 * nblk; ++i) {
+    if constexpr (!kE4m3) {
+      // ---- bf16 rows, sixteen lanes a row, straight into the swizzled operand layout (cp.async)
+      const int sub = lane >> 4, chunk = lane & 15;
+      const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 256;
+      uint32_t to[4];                                    // where this lane's chunk goes in rows 2i + sub
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = part + 2 * i + sub;
+        to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
+                (((chunk & 7) ^ (row & 7)) << 4);
+      }
+      Entry next = next_entry(true), after = next_entry(false);
+      while (next.valid) {
         const Entry e = next;
         next = after;
-        after = entry_of(i + 2);
-        const bool is_v = e.is_v;
-        ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
+        after = next_entry(false);
+        const int row = row_of(e);
+        ok = ok && mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const char* src = static_cast<const char*>(is_v ? a.v : a.k) + col;
-        int row = -1;                                    // no key: arrives as zeros
-        if (e.key < khi) {
-          if (e.row >= 0 && e.row < a.kv_tokens)
-            row = e.row;
-          else
-            atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-        }
+        const char* src = static_cast<const char*>(e.is_v ? a.v : a.k) + e.kh * 256 + chunk * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int tok = __shfl_sync(0xffffffffu, row, 2 * j + sub);
@@ -552,11 +636,95 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         }
         cp_async_arrive(&ctl.kv_full[st]);
         if (++st == kStages) st = 0, phase ^= 1u;
+        if (!next.valid) {                               // nothing held back
+          next = after.valid ? after : next_entry(true);
+          after = next_entry(false);
+        }
+      }
+    } else {
+      // ---- e4m3 rows: fetched three ring positions ahead (cp.async, 48 KB in flight; held in registers
+      // they were waited for all at once), widened to bf16 with their scales on the way into the
+      // operand layout.  The widened rows are exact, so from there on the two pools go the same way.
+      const int sub = lane >> 3, c = lane & 7;           // row 4j + sub, codes 16c .. 16c + 15
+      const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 128;
+      uint8_t* const to = smem + kSmemKv + (c >> 2) * kHalfBytes + (part + sub) * 128;
+      uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * (kRawSlots * L::kRawBytes);
+      int bytes[kRawSlots];                              // which byte of its word a row's exponent is
+      bool there[kRawSlots] = {false, false, false};
+      auto fetch = [&](const Entry& e, int i) {
+        const int row = row_of(e);
+        uint8_t* const at_raw = raw + i * L::kRawBytes;
+        const uint8_t* exps = (e.is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + e.kh;
+        bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 3u);
+        if (lane < L::kWarpRows) cp_async4(smem_u32(at_raw + L::kRawRows + lane * 4), exps - bytes[i], row < 0 ? 0 : 4);
+        const uint8_t* src = static_cast<const uint8_t*>(e.is_v ? a.v : a.k) + e.kh * 128 + c * 16;
+#pragma unroll
+        for (int j = 0; j < L::kWarpRows / 4; ++j) {
+          const int tok = __shfl_sync(0xffffffffu, row, 4 * j + sub);
+          cp_async16(smem_u32(at_raw + j * 512 + lane * 16), src + max(tok, 0) * row_stride, tok < 0 ? 0 : 16);
+        }
+      };
+      // Lanes of a row's second half widen and store their two chunks in the other order: no two lanes
+      // of a row store to the same bank.
+      const int flip = c >= 4 ? 1 : 0;
+      const int c0 = 2 * (c & 3) + flip;
+      auto store = [&](int i) {
+        ok = ok && mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const uint8_t* const at_raw = raw + i * L::kRawBytes;
+        const int exp_byte =
+            (*reinterpret_cast<const uint32_t*>(at_raw + L::kRawRows + (lane % L::kWarpRows) * 4) >> (8 * bytes[i])) & 255u;
+#pragma unroll
+        for (int g = 0; g < L::kWarpRows / 4; g += 2) {  // two loads' rows at a time, so that their chains overlap
+          uint2 codes[2][2];
+          int e[2];
+          uint32_t w[2][8];
+          bool seldom = false;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            codes[j][0] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + flip * 8);
+            codes[j][1] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + (flip ^ 1) * 8);
+            e[j] = __shfl_sync(0xffffffffu, exp_byte, 4 * (g + j) + sub);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            seldom |= widen16(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
+          if (__any_sync(0xffffffffu, seldom)) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              widen16_seldom(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint8_t* row = to + st * kTileBytes + (g + j) * 512;
+            const int key = (part + 4 * (g + j) + sub) & 7;   // the swizzle
+            *reinterpret_cast<uint4*>(row + ((c0 ^ key) << 4)) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+            *reinterpret_cast<uint4*>(row + ((c0 ^ 1 ^ key) << 4)) = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.kv_full[st]);
+        if (++st == kStages) st = 0, phase ^= 1u;
+      };
+      Entry next = next_entry(true);
+      while (ok && (next.valid || there[0] || there[1] || there[2])) {
+#pragma unroll
+        for (int i = 0; i < kRawSlots; ++i) {
+          // one group a position, empty ones too: all but the last two have landed, this one's among them
+          asm volatile("cp.async.wait_group 2;" ::: "memory");
+          if (there[i]) store(i);
+          there[i] = ok && next.valid;
+          if (there[i]) fetch(next, i);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (there[i] || !next.valid) next = next_entry(!there[0] && !there[1] && !there[2]);
+        }
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");   // nothing in flight when the CTA leaves
   } else if (warp < kLoadWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kControlRegs));
 
     if (warp == kPlanWarp && lane == 0) {
       // ---- the units of this part, in order, and their query tiles
@@ -770,7 +938,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     }
   } else {
     // ---- softmax: this thread's row of its stream
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
     const int s = (warp - kSoftmaxWarp) >> 2, r = tid & 127;
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + s * 128 + t_lane, t_o = tmem + 256 + s * 128 + t_lane;
@@ -1000,13 +1168,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
               const int kb = first + blk * kBlk;
               if (min(kb + kBlk, khi) <= unit_hi && kb >= unit_lo) continue;
               for (int key = max(kb, key_lo); key < min(kb + kBlk, key_hi); ++key) {
-                const uint32_t* x = static_cast<const uint32_t*>(v_row(a, o, key));
-                if (x == nullptr) continue;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                  const uint32_t w = x[c * 16 + i];
-                  if ((w & 0x7f80u) == 0x7f80u) v[2 * i] += __uint_as_float(w << 16);
-                  if ((w & 0x7f800000u) == 0x7f800000u) v[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
+                  const float2 x = value_pair<kE4m3>(a, o, key, c * 32 + 2 * i);
+                  if (!isfinite(x.x)) v[2 * i] += x.x;
+                  if (!isfinite(x.y)) v[2 * i + 1] += x.y;
                 }
               }
             }
@@ -1136,77 +1302,6 @@ chunk_join_kernel(const MacB200ChunkArgs a) {
   if (a.lse && k == 0) a.lse[to] = l == 0.f ? -INFINITY : (ms + log2f(l)) * 0.6931471805599453f;
 }
 
-// One warp per (row, query head); a lane holds dims [4l, 4l+4).
-template <bool kE4m3>
-__global__ void __launch_bounds__(kRowWarps * 32) chunk_rows_kernel(const MacB200ChunkArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t task = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
-  if (task >= static_cast<int64_t>(a.q_rows) * a.Hq) return;
-  const int row = static_cast<int>(task / a.Hq), hq = static_cast<int>(task - static_cast<int64_t>(row) * a.Hq);
-  const int kh = hq / (a.Hq / a.Hkv);
-  int b = -1;
-  for (int i = 0; i < a.B; ++i) {
-    const int64_t o0 = a.offsets[i], o1 = a.offsets[i + 1];
-    if (o0 < 0 || o1 < o0 || o1 > a.q_rows) {
-      if (lane == 0) atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-      continue;
-    }
-    if (row >= o0 && row < o1) b = i;
-  }
-  if (b < 0) return;
-  const int n = a.offsets[b + 1] - a.offsets[b];
-  int kv = a.kv_lens[b];
-  const int req = a.req_ids[b];
-  if (req < 0 || req >= a.req_to_token_rows || kv < 0 || kv > a.req_to_token_stride) {
-    if (lane == 0) atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-    kv = 0;
-  }
-  const int64_t p = static_cast<int64_t>(kv) - n + (row - a.offsets[b]);
-  int64_t j0 = a.window >= 0 ? p + 1 - a.window : 0;
-  if (j0 < 0) j0 = 0;
-  const int64_t j1 = kv > 0 ? p + 1 : 0;
-  const __nv_bfloat16* qp =
-      static_cast<const __nv_bfloat16*>(a.q) + row * a.q_stride0 + hq * 128 + lane * 4;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < 4; ++i) q[i] = __bfloat162float(qp[i]) * a.sm_scale;
-  float m = -INFINITY, l = 0.f;
-  const int32_t* table = a.req_to_token + static_cast<int64_t>(kv > 0 ? req : 0) * a.req_to_token_stride;
-  for (int64_t j = j0; j < j1; ++j) {
-    const int64_t tok = table[j];
-    float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (tok >= 0 && tok < a.kv_tokens) {
-      const int64_t at = tok * a.Hkv + kh;
-      if (kE4m3) {
-        const uint32_t kc = reinterpret_cast<const uint32_t*>(a.k)[at * 32 + lane];
-        const uint32_t vc = reinterpret_cast<const uint32_t*>(a.v)[at * 32 + lane];
-        const float ks = kv8_scale(a.k_exp[at]), vs = kv8_scale(a.v_exp[at]);
-        for (int i = 0; i < 2; ++i) {
-          const float2 kf = kv8_unpack2(kc >> (16 * i)), vf = kv8_unpack2(vc >> (16 * i));
-          k[2 * i] = kf.x * ks, k[2 * i + 1] = kf.y * ks;
-          v[2 * i] = vf.x * vs, v[2 * i + 1] = vf.y * vs;
-        }
-      } else {
-        const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(a.k) + at * 128 + lane * 4;
-        const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(a.v) + at * 128 + lane * 4;
-        for (int i = 0; i < 4; ++i) k[i] = __bfloat162float(kp[i]), v[i] = __bfloat162float(vp[i]);
-      }
-    } else if (lane == 0) {
-      atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-    }
-    float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float m2 = fmaxf(m, s);
-    const float r = m2 == -INFINITY ? 1.f : __expf(m - m2), w = m2 == -INFINITY ? 0.f : __expf(s - m2);
-    m = m2;
-    l = l * r + w;
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * r + w * v[i];
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* op = static_cast<__nv_bfloat16*>(a.out) + (static_cast<int64_t>(row) * a.Hq + hq) * 128 + lane * 4;
-  for (int i = 0; i < 4; ++i) op[i] = __float2bfloat16_rn(o[i] * inv);
-  if (a.lse && lane == 0) a.lse[static_cast<int64_t>(row) * a.Hq + hq] = l == 0.f ? -INFINITY : m + logf(l);
-}
-
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int64_t workspace_bytes(int sms) { return kCutBytes + 2 * static_cast<int64_t>(sms) * kSlotBytes; }
@@ -1230,15 +1325,17 @@ EncodeTiledFn encode_tiled_fn() {
 // Sets the kernel up on the current device, once: its shared memory, and the check that it was
 // built with the registers that its warps trade among themselves (a build with fewer would wait
 // for them for ever).
+template <bool kE4m3>
 int prepare_kernel(int device) {
   static std::atomic<int> ready[64];
   if (device >= 0 && device < 64 && ready[device].load(std::memory_order_acquire)) return MAC_B200_OK;
   cudaFuncAttributes attr{};
-  MAC_CUDA(cudaFuncGetAttributes(&attr, chunk_attention_kernel));
-  if (attr.numRegs < kLaunchRegs)
+  MAC_CUDA(cudaFuncGetAttributes(&attr, chunk_attention_kernel<kE4m3>));
+  if (attr.numRegs < Layout<kE4m3>::kLaunchRegs)
     return fail(MAC_B200_EUNSUPPORTED, "the chunk attention kernel was built with %d registers a thread",
                 attr.numRegs);
-  MAC_CUDA(cudaFuncSetAttribute(chunk_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  MAC_CUDA(cudaFuncSetAttribute(chunk_attention_kernel<kE4m3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Layout<kE4m3>::kBytes));
   if (device >= 0 && device < 64) ready[device].store(1, std::memory_order_release);
   return MAC_B200_OK;
 }
@@ -1272,30 +1369,27 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
   MAC_REQUIRE(a.workspace_bytes >= workspace_bytes(sms), "workspace holds %lld bytes, %lld are needed",
               static_cast<long long>(a.workspace_bytes), static_cast<long long>(workspace_bytes(sms)));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  if (e4m3) {
-    const int64_t blocks = (static_cast<int64_t>(a.q_rows) * a.Hq + kRowWarps - 1) / kRowWarps;
-    MAC_REQUIRE(blocks < (int64_t(1) << 31), "chunk problem too large");
-    chunk_rows_kernel<true><<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, stream>>>(a);
-  } else {
-    MAC_REQUIRE(sms <= kMaxCtas, "too many multiprocessors");
-    if (const int rc = prepare_kernel(device)) return rc;
-    EncodeTiledFn enc = encode_tiled_fn();
-    if (enc == nullptr) return fail(MAC_B200_EUNSUPPORTED, "cuTensorMapEncodeTiled is not available");
-    alignas(64) CUtensorMap q_map;
-    const cuuint32_t ones[3] = {1u, 1u, 1u};
-    const int G = a.Hq / a.Hkv;
-    const cuuint64_t q_dims[3] = {128u, static_cast<cuuint64_t>(a.Hq), static_cast<cuuint64_t>(a.q_rows)};
-    const cuuint64_t q_strides[2] = {256u, static_cast<cuuint64_t>(a.q_stride0) * 2};
-    const cuuint32_t q_box[3] = {64u, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(kRows / G)};
-    const CUresult rc = enc(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), q_dims, q_strides, q_box,
-                      ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                      CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (rc != CUDA_SUCCESS) return fail(MAC_B200_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
-    chunk_attention_kernel<<<sms, kThreads, kSmemBytes, stream>>>(a, q_map);
-    MAC_CUDA(cudaGetLastError());
-    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-    chunk_join_kernel<<<dim3(sms, 2 * kRows / kJoinRows), 256, 0, stream>>>(a);
-  }
+  MAC_REQUIRE(sms <= kMaxCtas, "too many multiprocessors");
+  if (const int rc = e4m3 ? prepare_kernel<true>(device) : prepare_kernel<false>(device)) return rc;
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return fail(MAC_B200_EUNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+  alignas(64) CUtensorMap q_map;                         // box: 64 dims x the G heads of a KV head x 128/G tokens
+  const cuuint32_t ones[3] = {1u, 1u, 1u};
+  const int G = a.Hq / a.Hkv;
+  const cuuint64_t q_dims[3] = {128u, static_cast<cuuint64_t>(a.Hq), static_cast<cuuint64_t>(a.q_rows)};
+  const cuuint64_t q_strides[2] = {256u, static_cast<cuuint64_t>(a.q_stride0) * 2};
+  const cuuint32_t q_box[3] = {64u, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(kRows / G)};
+  const CUresult rc = enc(&q_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), q_dims, q_strides,
+                          q_box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MAC_B200_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
+  if (e4m3)
+    chunk_attention_kernel<true><<<sms, Layout<true>::kThreads, Layout<true>::kBytes, stream>>>(a, q_map);
+  else
+    chunk_attention_kernel<false><<<sms, Layout<false>::kThreads, Layout<false>::kBytes, stream>>>(a, q_map);
+  MAC_CUDA(cudaGetLastError());
+  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  chunk_join_kernel<<<dim3(sms, 2 * kRows / kJoinRows), 256, 0, stream>>>(a);
   MAC_CUDA(cudaGetLastError());
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   return MAC_B200_OK;
