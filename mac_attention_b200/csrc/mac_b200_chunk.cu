@@ -395,23 +395,6 @@ __device__ __forceinline__ long long scan_cta(long long mine, long long& before,
 __device__ __forceinline__ int ring_v(int dual, int blk, int nblk) {
   return dual ? 2 * blk + 1 : min(2 * blk + 2, 2 * nblk - 1);
 }
-// and back: what ring position i holds
-__device__ __forceinline__ void ring_at(int dual, int nblk, int i, int& blk, bool& is_v) {
-  if (dual) {
-    blk = i >> 1;
-    is_v = i & 1;
-  } else if (i == 0) {
-    blk = 0;
-    is_v = false;
-  } else if (i & 1) {
-    blk = (i + 1) >> 1;
-    is_v = blk >= nblk;
-    if (is_v) blk = nblk - 1;
-  } else {
-    blk = (i - 2) >> 1;
-    is_v = true;
-  }
-}
 
 // Dims [d, d + 2) of the value of key `key`; zeros where the page table leads outside the pool.
 template <bool kE4m3>
@@ -554,171 +537,161 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     else
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kLoadRegs));
     const int part = (warp - kLoadWarp) * L::kWarpRows;  // this warp's rows of a block
-    // What the table says of row `lane` of this warp's part, and where its rows lie.  Entries are
-    // asked for ahead and looked at when they are needed.
-    struct Entry {
-      bool valid, exists, is_v;
-      int row, kh;
-    };
-    // The ring positions of this CTA's units, one after the other.  An entry that is not valid: there
-    // are no more (`more` is false), or the next unit is not announced yet.  A warp may wait for that
-    // only when it holds no position back: the announcement may wait for units that need it.
-    int it = 0, at = 0, dual = 0, nblk = 0, khi = 0, first = 0, kh = 0;
-    const int32_t* table = nullptr;
-    bool ok = true, more = true;
-    auto next_entry = [&](bool wait) {
-      Entry e{false, false, false, -1, 0};
-      while (more && at >= 2 * nblk) {                   // on to the next unit
-        const int slot = it & (kItems - 1);
-        if (wait)
-          ok = ok && mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
-        else if (!__all_sync(0xffffffffu, mbar_try(smem_u32(&ctl.item_full[slot]), (it / kItems) & 1)))
-          return e;
-        ok = __all_sync(0xffffffffu, ok);
-        const Item& o = ctl.items[slot];
-        more = ok && o.valid;
-        if (!more) break;
-        dual = o.dual;
-        nblk = o.nblk;
-        khi = o.khi;
-        first = o.k0 + o.blk0 * kBlk;
-        kh = o.kh;
-        table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
-        at = 0;
-        ++it;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
-      }
-      if (!more) return e;
-      int blk;
-      ring_at(dual, nblk, at++, blk, e.is_v);
-      const int key = first + blk * kBlk + part + lane;
-      e.valid = true;
-      e.exists = lane < L::kWarpRows && key < khi;
-      e.kh = kh;
-      if (e.exists) e.row = load_early(table + key);
-      return e;
-    };
-    // the pool row of an entry; -1: no key, or one outside the pool (reported): arrives as zeros
-    auto row_of = [&](const Entry& e) {
-      if (!e.exists) return -1;
-      if (e.row >= 0 && e.row < a.kv_tokens) return e.row;
-      atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-      return -1;
-    };
     uint32_t st = 0, phase = 1;                          // of the ring position to fill next
+    bool ok = true;
+    // bf16: sixteen lanes a row, straight into the swizzled operand layout (cp.async).
+    // e4m3: eight lanes a row, three ring positions ahead into a raw buffer (48 KB in flight; held in
+    // registers they were waited for all at once), then widened to bf16 with their scales on the way
+    // into the operand layout.  The widened rows are exact: from there on the two pools go the same way.
+    constexpr int kLanes = kE4m3 ? 8 : 16, kPerLoad = 32 / kLanes;   // lanes a row, rows a load
+    const int sub = lane / kLanes, c = lane % kLanes;    // row kPerLoad * j + sub of the part, 16 bytes of it
+    const int64_t row_stride = static_cast<int64_t>(a.Hkv) * (kE4m3 ? 128 : 256);
+    uint32_t to[4];                                      // bf16: where this lane's chunk goes in rows 2i + sub
     if constexpr (!kE4m3) {
-      // ---- bf16 rows, sixteen lanes a row, straight into the swizzled operand layout (cp.async)
-      const int sub = lane >> 4, chunk = lane & 15;
-      const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 256;
-      uint32_t to[4];                                    // where this lane's chunk goes in rows 2i + sub
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = part + 2 * i + sub;
-        to[i] = smem_u32(smem + kSmemKv) + (chunk >> 3) * kHalfBytes + row * 128 +
-                (((chunk & 7) ^ (row & 7)) << 4);
+        to[i] = smem_u32(smem + kSmemKv) + (c >> 3) * kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
       }
-      Entry next = next_entry(true), after = next_entry(false);
-      while (next.valid) {
-        const Entry e = next;
-        next = after;
-        after = next_entry(false);
-        const int row = row_of(e);
-        ok = ok && mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const char* src = static_cast<const char*>(e.is_v ? a.v : a.k) + e.kh * 256 + chunk * 16;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int tok = __shfl_sync(0xffffffffu, row, 2 * j + sub);
-          cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes,
-                     src + (tok < 0 ? 0 : tok) * row_stride, tok < 0 ? 0 : 16);
-        }
-        cp_async_arrive(&ctl.kv_full[st]);
-        if (++st == kStages) st = 0, phase ^= 1u;
-        if (!next.valid) {                               // nothing held back
-          next = after.valid ? after : next_entry(true);
-          after = next_entry(false);
-        }
-      }
-    } else {
-      // ---- e4m3 rows: fetched three ring positions ahead (cp.async, 48 KB in flight; held in registers
-      // they were waited for all at once), widened to bf16 with their scales on the way into the
-      // operand layout.  The widened rows are exact, so from there on the two pools go the same way.
-      const int sub = lane >> 3, c = lane & 7;           // row 4j + sub, codes 16c .. 16c + 15
-      const int64_t row_stride = static_cast<int64_t>(a.Hkv) * 128;
-      uint8_t* const to = smem + kSmemKv + (c >> 2) * kHalfBytes + (part + sub) * 128;
-      uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * (kRawSlots * L::kRawBytes);
-      int bytes[kRawSlots];                              // which byte of its word a row's exponent is
-      bool there[kRawSlots] = {false, false, false};
-      auto fetch = [&](const Entry& e, int i) {
-        const int row = row_of(e);
-        uint8_t* const at_raw = raw + i * L::kRawBytes;
-        const uint8_t* exps = (e.is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + e.kh;
-        bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 3u);
-        if (lane < L::kWarpRows) cp_async4(smem_u32(at_raw + L::kRawRows + lane * 4), exps - bytes[i], row < 0 ? 0 : 4);
-        const uint8_t* src = static_cast<const uint8_t*>(e.is_v ? a.v : a.k) + e.kh * 128 + c * 16;
-#pragma unroll
-        for (int j = 0; j < L::kWarpRows / 4; ++j) {
-          const int tok = __shfl_sync(0xffffffffu, row, 4 * j + sub);
-          cp_async16(smem_u32(at_raw + j * 512 + lane * 16), src + max(tok, 0) * row_stride, tok < 0 ? 0 : 16);
-        }
+    }
+    uint8_t* const wide = smem + kSmemKv + (c >> 2) * kHalfBytes + (part + sub) * 128;   // e4m3: the same, widened
+    uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * (kRawSlots * L::kRawBytes);
+    int bytes[kRawSlots];                                // which byte of its word a row's exponent is
+    for (int it = 0; ok; ++it) {
+      const int slot = it & (kItems - 1);
+      ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const Item& o = ctl.items[slot];
+      if (!o.valid) break;
+      const int dual = o.dual, nblk = o.nblk, khi = o.khi, kh = o.kh;
+      const int first = o.k0 + o.blk0 * kBlk;
+      const int64_t col = kh * (kE4m3 ? 128 : 256) + c * 16;
+      const int32_t* table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
+      // Key `lane` of this warp's part of the next ring position: the key, and what the table says of
+      // it.  Table entries are asked for ahead and looked at when they are needed.
+      struct Entry {
+        int key, row;
+        bool is_v;
       };
-      // Lanes of a row's second half widen and store their two chunks in the other order: no two lanes
-      // of a row store to the same bank.
-      const int flip = c >= 4 ? 1 : 0;
-      const int c0 = 2 * (c & 3) + flip;
-      auto store = [&](int i) {
-        ok = ok && mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        const uint8_t* const at_raw = raw + i * L::kRawBytes;
-        const int exp_byte =
-            (*reinterpret_cast<const uint32_t*>(at_raw + L::kRawRows + (lane % L::kWarpRows) * 4) >> (8 * bytes[i])) & 255u;
+      int k_next = 0, v_next = 0;                        // blocks asked for; see ring_v()
+      auto entry_of = [&]() {
+        Entry e{khi, 0, false};
+        if (v_next == nblk) return e;
+        e.is_v = k_next == nblk || k_next > v_next + (dual ? 0 : 1);
+        e.key = first + (e.is_v ? v_next++ : k_next++) * kBlk + part + lane;
+        if (lane >= L::kWarpRows) e.key = khi;
+        if (e.key < khi) e.row = load_early(table + e.key);
+        return e;
+      };
+      // the pool row; -1: no key, or one outside the pool (reported): arrives as zeros
+      auto row_of = [&](const Entry& e) {
+        if (e.key >= khi) return -1;
+        if (e.row >= 0 && e.row < a.kv_tokens) return e.row;
+        atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+        return -1;
+      };
+      Entry next = entry_of(), after = entry_of();
+      if constexpr (!kE4m3) {
+        for (int i = 0; i < 2 * nblk; ++i) {
+          const Entry e = next;
+          next = after;
+          after = entry_of();
+          ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const char* src = static_cast<const char*>(e.is_v ? a.v : a.k) + col;
+          const int row = row_of(e);
 #pragma unroll
-        for (int g = 0; g < L::kWarpRows / 4; g += 2) {  // two loads' rows at a time, so that their chains overlap
-          uint2 codes[2][2];
-          int e[2];
-          uint32_t w[2][8];
-          bool seldom = false;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            codes[j][0] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + flip * 8);
-            codes[j][1] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + (flip ^ 1) * 8);
-            e[j] = __shfl_sync(0xffffffffu, exp_byte, 4 * (g + j) + sub);
+          for (int j = 0; j < 16; ++j) {
+            const int tok = __shfl_sync(0xffffffffu, row, 2 * j + sub);
+            cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes, src + (tok < 0 ? 0 : tok) * row_stride,
+                       tok < 0 ? 0 : 16);
           }
+          cp_async_arrive(&ctl.kv_full[st]);
+          if (++st == kStages) st = 0, phase ^= 1u;
+        }
+      } else {
+        auto fetch = [&](const Entry& e, int i) {
+          const int row = row_of(e);
+          uint8_t* const at_raw = raw + i * L::kRawBytes;
+          const uint8_t* exps = (e.is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + kh;
+          bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 3u);
+          if (lane < L::kWarpRows)
+            cp_async4(smem_u32(at_raw + L::kRawRows + lane * 4), exps - bytes[i], row < 0 ? 0 : 4);
+          const uint8_t* src = static_cast<const uint8_t*>(e.is_v ? a.v : a.k) + col;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            seldom |= widen16(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
-          if (__any_sync(0xffffffffu, seldom)) {
+          for (int j = 0; j < L::kWarpRows / 4; ++j) {
+            const int tok = __shfl_sync(0xffffffffu, row, 4 * j + sub);
+            cp_async16(smem_u32(at_raw + j * 512 + lane * 16), src + max(tok, 0) * row_stride, tok < 0 ? 0 : 16);
+          }
+        };
+        // Lanes of a row's second half widen and store their two chunks in the other order: no two lanes
+        // of a row store to the same bank.
+        const int flip = c >= 4 ? 1 : 0;
+        const int c0 = 2 * (c & 3) + flip;
+        auto store = [&](int i) {
+          ok = ok && mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          const uint8_t* const at_raw = raw + i * L::kRawBytes;
+          const int exp_byte =
+              (*reinterpret_cast<const uint32_t*>(at_raw + L::kRawRows + (lane % L::kWarpRows) * 4) >> (8 * bytes[i])) & 255u;
+#pragma unroll
+          for (int g = 0; g < L::kWarpRows / 4; g += 2) {  // two loads' rows at a time, so that their chains overlap
+            uint2 codes[2][2];
+            int e[2];
+            uint32_t w[2][8];
+            bool seldom = false;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              codes[j][0] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + flip * 8);
+              codes[j][1] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + (flip ^ 1) * 8);
+              e[j] = __shfl_sync(0xffffffffu, exp_byte, 4 * (g + j) + sub);
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              widen16_seldom(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
-          }
+              seldom |= widen16(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
+            if (__any_sync(0xffffffffu, seldom)) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint8_t* row = to + st * kTileBytes + (g + j) * 512;
-            const int key = (part + 4 * (g + j) + sub) & 7;   // the swizzle
-            *reinterpret_cast<uint4*>(row + ((c0 ^ key) << 4)) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
-            *reinterpret_cast<uint4*>(row + ((c0 ^ 1 ^ key) << 4)) = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
+              for (int j = 0; j < 2; ++j)
+                widen16_seldom(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint8_t* row = wide + st * kTileBytes + (g + j) * 512;
+              const int key = (part + 4 * (g + j) + sub) & 7;   // the swizzle
+              *reinterpret_cast<uint4*>(row + ((c0 ^ key) << 4)) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+              *reinterpret_cast<uint4*>(row + ((c0 ^ 1 ^ key) << 4)) = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
+            }
           }
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.kv_full[st]);
-        if (++st == kStages) st = 0, phase ^= 1u;
-      };
-      Entry next = next_entry(true);
-      while (ok && (next.valid || there[0] || there[1] || there[2])) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.kv_full[st]);
+          if (++st == kStages) st = 0, phase ^= 1u;
+        };
+        const int n = 2 * nblk;
 #pragma unroll
         for (int i = 0; i < kRawSlots; ++i) {
-          // one group a position, empty ones too: all but the last two have landed, this one's among them
-          asm volatile("cp.async.wait_group 2;" ::: "memory");
-          if (there[i]) store(i);
-          there[i] = ok && next.valid;
-          if (there[i]) fetch(next, i);
+          if (i < n) fetch(next, i);
+          next = after;
+          after = entry_of();
           asm volatile("cp.async.commit_group;" ::: "memory");
-          if (there[i] || !next.valid) next = next_entry(!there[0] && !there[1] && !there[2]);
+        }
+        for (int i0 = 0; i0 < n && ok; i0 += kRawSlots) {
+#pragma unroll
+          for (int i = 0; i < kRawSlots; ++i) {
+            if (i0 + i >= n || !ok) break;
+            // one group a position, empty ones too: all but the last two have landed, this one's among them
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            store(i);
+            if (i0 + i + kRawSlots < n) fetch(next, i);
+            next = after;
+            after = entry_of();
+            asm volatile("cp.async.commit_group;" ::: "memory");
+          }
         }
       }
     }
@@ -858,17 +831,15 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
             q_phase[i] ^= 1u;
             if ((i != buf || n == 0) && lane == 0) mbar_arrive(&ctl.q_empty[i]);
           }
-        int at = 0;                                      // the next position within the unit
+        int at = 0, k_next = 0, v_next = 0;              // positions of the unit waited for; single: K, V blocks
         // waits for the stream's next own position; its stage, or -1
         auto next_stage = [&]() {
           while (ok) {
             ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
             bool mine = true;
             if (!dual) {
-              int blk;
-              bool is_v;
-              ring_at(0, nblk, at, blk, is_v);
-              mine = (blk & 1) == s;
+              const bool is_v = k_next == nblk || k_next > v_next + 1;
+              mine = ((is_v ? v_next++ : k_next++) & 1) == s;
               if (!mine && lane == 0) mbar_arrive(&ctl.kv_empty[st]);
             }
             const int found = static_cast<int>(st);
