@@ -119,7 +119,9 @@ struct Layout {
   static constexpr int kWarpRows = kBlk / kLoadWarps;    // rows of a block that a loading warp fetches
   static constexpr int kStages = kE4m3 ? 3 : kMaxStages;
   static constexpr int kRawRows = kWarpRows * 128;       // of a warp and a ring position
-  static constexpr int kRawBytes = kRawRows + kWarpRows * 4;   // and the words that hold the exponents
+  // with the words that hold the rows' exponents, and the table's entries of three positions later
+  static constexpr int kRawExps = kRawRows, kRawEntries = kRawExps + kWarpRows * 4;
+  static constexpr int kRawBytes = kRawEntries + kWarpRows * 4;
   static constexpr int kRaw = kSmemKv + kStages * kTileBytes;
   static constexpr int kControl = kRaw + (kE4m3 ? kRawSlots * kLoadWarps * kRawBytes : 0);
   static constexpr int kBytes = kControl + static_cast<int>(sizeof(Control));
@@ -416,32 +418,23 @@ __device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
   __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// Sixteen codes of a row to bf16 (eight words), without a branch, and whether that was not enough.
-// An e4m3 number's exponent and mantissa bits, moved to where bf16 has its own, read as the number
-// times 2^-120 (the difference of the biases), subnormal codes included; one factor puts the row's
-// scale on, exactly.  Not enough: codes of NaN, and rows whose factor would overflow (past 448 * 2^7).
-__device__ __forceinline__ bool widen16(const uint4& c, int e, uint32_t (&w)[8]) {
-  const uint32_t code[4] = {c.x, c.y, c.z, c.w};
-  const uint32_t f = e == kKv8NanExp ? 0x7fc0u : static_cast<uint32_t>(min(e, 134) + 120) << 7;
-  const uint32_t f2 = f | (f << 16);
-  uint32_t odd = 0u;
+// A row's scale as a pair of bf16: 2^(e-127), NaN for e = 255.
+__device__ __forceinline__ uint32_t scale_pair(int e) {
+  const uint32_t f = e == kKv8NanExp ? 0x7fc0u : e == 0 ? 0x0040u : static_cast<uint32_t>(e) << 7;
+  return f | (f << 16);
+}
+// Eight codes of a row to bf16 (four words): through fp16 and fp32, which hold every code, to bf16,
+// which does too, and then the scale, a power of two.  (200 cycles a warp for 64 codes a lane;
+// moving the bits by hand took 290 and a check for codes of NaN beside it.)
+__device__ __forceinline__ uint4 widen8(const uint2& codes, uint32_t scale) {
+  const uint32_t c[2] = {codes.x, codes.y};
+  uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t x = __byte_perm(code[i], 0u, 0x1404), y = __byte_perm(code[i], 0u, 0x3424);
-    w[2 * i] = mul_bf16(((x >> 4) & 0x07f007f0u) | (x & 0x80008000u), f2);
-    w[2 * i + 1] = mul_bf16(((y >> 4) & 0x07f007f0u) | (y & 0x80008000u), f2);
-    odd |= (code[i] & 0x7f7f7f7fu) + 0x01010101u;
+    const float2 x = kv8_unpack2(c[i >> 1] >> ((i & 1) * 16));
+    w[i] = mul_bf16(pack_bf16(x.x, x.y), scale);
   }
-  return (odd & 0x80808080u) != 0u || (e > 134 && e != kKv8NanExp);
-}
-__device__ __forceinline__ void widen16_seldom(const uint4& c, int e, uint32_t (&w)[8]) {
-  const uint32_t code[4] = {c.x, c.y, c.z, c.w};
-  const float s = kv8_scale(e);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 x = kv8_unpack2(code[i >> 1] >> ((i & 1) * 16));
-    w[i] = pack_bf16(x.x * s, x.y * s);
-  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <bool kE4m3>
@@ -583,7 +576,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         e.is_v = k_next == nblk || k_next > v_next + (dual ? 0 : 1);
         e.key = first + (e.is_v ? v_next++ : k_next++) * kBlk + part + lane;
         if (lane >= L::kWarpRows) e.key = khi;
-        if (e.key < khi) e.row = load_early(table + e.key);
+        if (!kE4m3 && e.key < khi) e.row = load_early(table + e.key);
         return e;
       };
       // the pool row; -1: no key, or one outside the pool (reported): arrives as zeros
@@ -593,25 +586,28 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
         return -1;
       };
-      Entry next = entry_of(), after = entry_of();
+      // Entries are refilled where they were used: moved on to another one they would be waited for.
+      const int n = 2 * nblk;
       if constexpr (!kE4m3) {
-        for (int i = 0; i < 2 * nblk; ++i) {
-          const Entry e = next;
-          next = after;
-          after = entry_of();
-          ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const char* src = static_cast<const char*>(e.is_v ? a.v : a.k) + col;
-          const int row = row_of(e);
+        Entry e[2] = {entry_of(), entry_of()};
+        for (int i0 = 0; i0 < n && ok; i0 += 2) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int tok = __shfl_sync(0xffffffffu, row, 2 * j + sub);
-            cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes, src + (tok < 0 ? 0 : tok) * row_stride,
-                       tok < 0 ? 0 : 16);
+          for (int i = 0; i < 2; ++i) {                  // n is even
+            ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const char* src = static_cast<const char*>(e[i].is_v ? a.v : a.k) + col;
+            const int row = row_of(e[i]);
+            e[i] = entry_of();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int tok = __shfl_sync(0xffffffffu, row, 2 * j + sub);
+              cp_async16(to[j & 3] + (j >> 2) * 1024 + st * kTileBytes, src + (tok < 0 ? 0 : tok) * row_stride,
+                         tok < 0 ? 0 : 16);
+            }
+            cp_async_arrive(&ctl.kv_full[st]);
+            if (++st == kStages) st = 0, phase ^= 1u;
           }
-          cp_async_arrive(&ctl.kv_full[st]);
-          if (++st == kStages) st = 0, phase ^= 1u;
         }
       } else {
         auto fetch = [&](const Entry& e, int i) {
@@ -620,7 +616,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           const uint8_t* exps = (e.is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + kh;
           bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 3u);
           if (lane < L::kWarpRows)
-            cp_async4(smem_u32(at_raw + L::kRawRows + lane * 4), exps - bytes[i], row < 0 ? 0 : 4);
+            cp_async4(smem_u32(at_raw + L::kRawExps + lane * 4), exps - bytes[i], row < 0 ? 0 : 4);
           const uint8_t* src = static_cast<const uint8_t*>(e.is_v ? a.v : a.k) + col;
 #pragma unroll
           for (int j = 0; j < L::kWarpRows / 4; ++j) {
@@ -637,59 +633,63 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           const uint8_t* const at_raw = raw + i * L::kRawBytes;
-          const int exp_byte =
-              (*reinterpret_cast<const uint32_t*>(at_raw + L::kRawRows + (lane % L::kWarpRows) * 4) >> (8 * bytes[i])) & 255u;
+          const uint32_t exp_word = *reinterpret_cast<const uint32_t*>(at_raw + L::kRawExps + (lane % L::kWarpRows) * 4);
+          const uint32_t scale_own = scale_pair((exp_word >> (8 * bytes[i])) & 255u);
+          // everything is read before anything is stored: the compiler keeps reads behind stores that it
+          // cannot tell apart from them
+          uint2 codes[L::kWarpRows / 4][2];
+          uint32_t scale_row[L::kWarpRows / 4];
 #pragma unroll
-          for (int g = 0; g < L::kWarpRows / 4; g += 2) {  // two loads' rows at a time, so that their chains overlap
-            uint2 codes[2][2];
-            int e[2];
-            uint32_t w[2][8];
-            bool seldom = false;
+          for (int j = 0; j < L::kWarpRows / 4; ++j) {
+            codes[j][0] = *reinterpret_cast<const uint2*>(at_raw + j * 512 + lane * 16 + flip * 8);
+            codes[j][1] = *reinterpret_cast<const uint2*>(at_raw + j * 512 + lane * 16 + (flip ^ 1) * 8);
+            scale_row[j] = __shfl_sync(0xffffffffu, scale_own, 4 * j + sub);
+          }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              codes[j][0] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + flip * 8);
-              codes[j][1] = *reinterpret_cast<const uint2*>(at_raw + (g + j) * 512 + lane * 16 + (flip ^ 1) * 8);
-              e[j] = __shfl_sync(0xffffffffu, exp_byte, 4 * (g + j) + sub);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              seldom |= widen16(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
-            if (__any_sync(0xffffffffu, seldom)) {
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                widen16_seldom(make_uint4(codes[j][0].x, codes[j][0].y, codes[j][1].x, codes[j][1].y), e[j], w[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint8_t* row = wide + st * kTileBytes + (g + j) * 512;
-              const int key = (part + 4 * (g + j) + sub) & 7;   // the swizzle
-              *reinterpret_cast<uint4*>(row + ((c0 ^ key) << 4)) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
-              *reinterpret_cast<uint4*>(row + ((c0 ^ 1 ^ key) << 4)) = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
-            }
+          for (int j = 0; j < L::kWarpRows / 4; ++j) {
+            uint8_t* row = wide + st * kTileBytes + j * 512;
+            const int key = (part + 4 * j + sub) & 7;    // the swizzle
+            *reinterpret_cast<uint4*>(row + ((c0 ^ key) << 4)) = widen8(codes[j][0], scale_row[j]);
+            *reinterpret_cast<uint4*>(row + ((c0 ^ 1 ^ key) << 4)) = widen8(codes[j][1], scale_row[j]);
           }
           fence_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.kv_full[st]);
           if (++st == kStages) st = 0, phase ^= 1u;
         };
-        const int n = 2 * nblk;
+        // Table entries come by cp.async too: a load into a register shares its scoreboard with the
+        // loads of the widening, which would wait for it.
+        Entry e[kRawSlots];
+        auto ask = [&](int i) {
+          e[i] = entry_of();
+          if (e[i].key < khi)
+            cp_async4(smem_u32(raw + i * L::kRawBytes + L::kRawEntries + lane * 4), table + e[i].key, 4);
+        };
+        auto asked = [&](int i) {
+          if (e[i].key < khi)
+            e[i].row = *reinterpret_cast<const int*>(raw + i * L::kRawBytes + L::kRawEntries + lane * 4);
+        };
+#pragma unroll
+        for (int i = 0; i < kRawSlots; ++i) ask(i);
+        asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < kRawSlots; ++i) {
-          if (i < n) fetch(next, i);
-          next = after;
-          after = entry_of();
+          asked(i);
+          if (i < n) fetch(e[i], i);
+          ask(i);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
         for (int i0 = 0; i0 < n && ok; i0 += kRawSlots) {
 #pragma unroll
           for (int i = 0; i < kRawSlots; ++i) {
             if (i0 + i >= n || !ok) break;
-            // one group a position, empty ones too: all but the last two have landed, this one's among them
+            // one group a position, empty ones too: all but the last two have landed, this position's
+            // rows and the entries of the one three later among them
             asm volatile("cp.async.wait_group 2;" ::: "memory");
+            asked(i);
             store(i);
-            if (i0 + i + kRawSlots < n) fetch(next, i);
-            next = after;
-            after = entry_of();
+            if (i0 + i + kRawSlots < n) fetch(e[i], i);
+            ask(i);
             asm volatile("cp.async.commit_group;" ::: "memory");
           }
         }
