@@ -31,6 +31,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -119,8 +120,8 @@ struct Layout {
   static constexpr int kWarpRows = kBlk / kLoadWarps;    // rows of a block that a loading warp fetches
   static constexpr int kStages = kE4m3 ? 3 : kMaxStages;
   static constexpr int kRawRows = kWarpRows * 128;       // of a warp and a ring position
-  // with the words that hold the rows' exponents, and the table's entries of three positions later
-  static constexpr int kRawExps = kRawRows, kRawEntries = kRawExps + kWarpRows * 4;
+  // with the 16 bytes around each row's exponent, and the table's entries of three positions later
+  static constexpr int kRawExps = kRawRows, kRawEntries = kRawExps + kWarpRows * 16;
   static constexpr int kRawBytes = kRawEntries + kWarpRows * 4;
   static constexpr int kRaw = kSmemKv + kStages * kTileBytes;
   static constexpr int kControl = kRaw + (kE4m3 ? kRawSlots * kLoadWarps * kRawBytes : 0);
@@ -441,6 +442,8 @@ template <bool kE4m3>
 __global__ void __launch_bounds__(Layout<kE4m3>::kThreads, 1)
 chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtensorMap q_map) {
   extern __shared__ __align__(1024) uint8_t smem[];      // the swizzle repeats every 1024 bytes
+  // the joining kernel may be set up from here on; it waits for this one's end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using L = Layout<kE4m3>;
   constexpr int kStages = L::kStages, kThreads = L::kThreads, kLoadWarps = L::kLoadWarps;
   constexpr int kSoftmaxWarp = L::kSoftmaxWarp;
@@ -549,7 +552,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     }
     uint8_t* const wide = smem + kSmemKv + (c >> 2) * kHalfBytes + (part + sub) * 128;   // e4m3: the same, widened
     uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * (kRawSlots * L::kRawBytes);
-    int bytes[kRawSlots];                                // which byte of its word a row's exponent is
+    int bytes[kRawSlots];                                // which of its 16 bytes a row's exponent is
     for (int it = 0; ok; ++it) {
       const int slot = it & (kItems - 1);
       ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
@@ -614,9 +617,13 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           const int row = row_of(e);
           uint8_t* const at_raw = raw + i * L::kRawBytes;
           const uint8_t* exps = (e.is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + kh;
-          bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 3u);
+          bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 15u);
+          const uint8_t* const end = (e.is_v ? a.v_exp : a.k_exp) + a.kv_tokens * a.Hkv;
+          // 16-byte copies pass the L1 cache by; single words would each hold a line of the little that
+          // this much shared memory leaves of it, and wait for one
           if (lane < L::kWarpRows)
-            cp_async4(smem_u32(at_raw + L::kRawExps + lane * 4), exps - bytes[i], row < 0 ? 0 : 4);
+            cp_async16(smem_u32(at_raw + L::kRawExps + lane * 16), exps - bytes[i],
+                       row < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), end - (exps - bytes[i]))));
           const uint8_t* src = static_cast<const uint8_t*>(e.is_v ? a.v : a.k) + col;
 #pragma unroll
           for (int j = 0; j < L::kWarpRows / 4; ++j) {
@@ -633,8 +640,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           const uint8_t* const at_raw = raw + i * L::kRawBytes;
-          const uint32_t exp_word = *reinterpret_cast<const uint32_t*>(at_raw + L::kRawExps + (lane % L::kWarpRows) * 4);
-          const uint32_t scale_own = scale_pair((exp_word >> (8 * bytes[i])) & 255u);
+          const uint32_t scale_own = scale_pair(at_raw[L::kRawExps + (lane % L::kWarpRows) * 16 + bytes[i]]);
           // everything is read before anything is stored: the compiler keeps reads behind stores that it
           // cannot tell apart from them
           uint2 codes[L::kWarpRows / 4][2];
@@ -1199,6 +1205,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
 // run in an order that the parts and rows alone decide.
 __global__ void __launch_bounds__(256)
 chunk_join_kernel(const MacB200ChunkArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Cut cut = static_cast<const Cut*>(a.workspace)[blockIdx.x];
   const int G = a.Hq / a.Hkv, tile_tokens = kRows / G;
   const int row_first = blockIdx.y * kJoinRows, rows = min(cut.ntok * G - row_first, kJoinRows);
@@ -1360,7 +1367,17 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
     chunk_attention_kernel<false><<<sms, Layout<false>::kThreads, Layout<false>::kBytes, stream>>>(a, q_map);
   MAC_CUDA(cudaGetLastError());
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-  chunk_join_kernel<<<dim3(sms, 2 * kRows / kJoinRows), 256, 0, stream>>>(a);
+  cudaLaunchConfig_t config{};
+  const int most_rows = std::min(a.q_rows, 2 * (kRows / G)) * G;   // of a unit
+  config.gridDim = dim3(static_cast<unsigned>(sms), static_cast<unsigned>((most_rows + kJoinRows - 1) / kJoinRows));
+  config.blockDim = dim3(256);
+  config.stream = stream;
+  cudaLaunchAttribute early{};                           // set up while the first kernel runs
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  MAC_CUDA(cudaLaunchKernelEx(&config, chunk_join_kernel, a));
   MAC_CUDA(cudaGetLastError());
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   return MAC_B200_OK;
