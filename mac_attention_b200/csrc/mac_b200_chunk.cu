@@ -53,7 +53,7 @@ constexpr int kItems = 4;                  // units announced ahead
 // Warps by role.  The issuing warps come first: a scheduler prefers its older warps.
 constexpr int kMmaWarp = 0, kPlanWarp = 2, kLoadWarp = 4, kSoftmaxWarps = 8;
 constexpr int kUnitCells = 1;              // what a unit costs beside its blocks, in blocks
-constexpr int kMinCells = 3;               // least work worth a CTA of its own, where units are long
+constexpr int kMinCells = 2;               // least work worth a CTA of its own (1, 4, 6: up to 5 us slower)
 constexpr int kJoinRows = 16;              // rows of a unit that a block of the second kernel joins
 constexpr int kTmemCols = 512;             // S0 S1 O0 O1; the weights lie over the scores
 constexpr long long kWaitLimitClocks = 4000000000ll;   // about two seconds
@@ -457,14 +457,16 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   const int per = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
   long long mine = 0, before;
+  const Request mine0 = b0 < b1 ? load_request(a, b0, blockIdx.x == 0) : Request{};   // most calls: a thread's only one
   for (int b = b0; b < b1; ++b)
-    mine += a.Hkv * static_cast<long long>((load_request(a, b, blockIdx.x == 0).n + tile_tokens - 1) / tile_tokens);
+    mine += a.Hkv * static_cast<long long>(
+                        ((b == b0 ? mine0 : load_request(a, b, blockIdx.x == 0)).n + tile_tokens - 1) / tile_tokens);
   // pairs of tiles once there are enough of them for every CTA
   const int span = scan_cta<kThreads>(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
   long long units = 0;
   mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const Request r = load_request(a, b, false);
+    const Request r = b == b0 ? mine0 : load_request(a, b, false);
     mine += a.Hkv * head_cells(r, a.window, span);
     units += a.Hkv * static_cast<long long>((r.n + span - 1) / span);
   }
@@ -482,7 +484,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   if (lo >= before && lo < before + mine) {
     long long at = before;
     for (int b = b0; b < b1; ++b) {
-      const long long len = a.Hkv * head_cells(load_request(a, b, false), a.window, span);
+      const long long len = a.Hkv * head_cells(b == b0 ? mine0 : load_request(a, b, false), a.window, span);
       if (lo < at + len) {
         ctl.start_b = b;
         ctl.start_pos = at;

@@ -2,8 +2,8 @@
 // and read back (sm_100a).  Format and rules: include/mac_b200_chunk.h.
 //
 // Both directions are memory streams: a row of 128 values is 256 bytes in bf16 and 129 held.
-// Eight lanes own a row, 16 values each: a lane's two 16-byte loads are issued before anything is
-// computed, the row's maximum is three shuffles away, and the codes leave as one 16-byte store a
+// Eight lanes own a row of k and the row of v beside it, 16 values of each: a lane's four 16-byte
+// loads are issued before anything is computed, a row's maximum is three shuffles away, and the codes leave as one 16-byte store a
 // lane (128 bytes a row).  Under the half-split rotation a lane owns dims [8l, 8l+8) and
 // [64+8l, 64+8l+8) instead, so both members of a pair are in one thread; its codes leave as two
 // 8-byte stores.  The row's exponent is found from the bits of its maximum, no logarithm.
@@ -125,36 +125,38 @@ __device__ __forceinline__ void rotate_row(const MacB200QuantizeKvArgs& a, const
   }
 }
 
-// One task = one row of one token: its k heads, its v heads and (kRope) its q heads, in that order.
+// One task = one KV head of one token, its k row and its v row (four loads a lane before anything is
+// computed), or with kRope one query head, after the KV heads.
 // kVec: rows are 16-byte aligned (and under kSplit the whole row is rotated in split pairs).
 template <bool kRope, bool kSplit, bool kVec>
 __global__ void __launch_bounds__(kKv8Threads) kv8_write_kernel(const MacB200QuantizeKvArgs a) {
-  const int heads = 2 * a.Hkv + (kRope ? a.Hq : 0);
+  const int heads = a.Hkv + (kRope ? a.Hq : 0);
   const int64_t tasks = a.N * heads;
   const int64_t t = (static_cast<int64_t>(blockIdx.x) * kKv8Threads + threadIdx.x) >> 3;
   const int lane8 = threadIdx.x & 7;
   const bool live = t < tasks;                       // whole groups of eight; the shuffles need every lane
   const int64_t n = live ? t / heads : 0;
   int h = live ? static_cast<int>(t - n * heads) : 0;
-  const bool is_v = h >= a.Hkv && h < 2 * a.Hkv, is_q = kRope && h >= 2 * a.Hkv;
-  if (is_v) h -= a.Hkv;
-  if (is_q) h -= 2 * a.Hkv;
-  const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(is_q ? a.q : is_v ? a.v : a.k);
-  const int64_t stride = is_q ? a.q_stride0 : is_v ? a.v_stride0 : a.k_stride0;
-  const __nv_bfloat16* row = src + n * stride + static_cast<int64_t>(h) * 128;
-  float x[16] = {};
+  const bool is_q = kRope && h >= a.Hkv;
+  if (is_q) h -= a.Hkv;
+  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(is_q ? a.q : a.k) +
+                             n * (is_q ? a.q_stride0 : a.k_stride0) + static_cast<int64_t>(h) * 128;
+  float x[16] = {}, y[16] = {};
   int64_t loc = -1, pos = 0;
   if (live) {
     load_row<kSplit, kVec>(row, lane8, x);
-    if (!is_q) loc = load_loc(a.cache_locs, a.cache_locs_i64, n);
+    if (!is_q) {
+      load_row<kSplit, kVec>(static_cast<const __nv_bfloat16*>(a.v) + n * a.v_stride0 + static_cast<int64_t>(h) * 128,
+                             lane8, y);
+      loc = load_loc(a.cache_locs, a.cache_locs_i64, n);
+    }
     if (kRope) pos = load_loc(a.positions, a.positions_i64, n);
   }
   bool ok = live;
   if (kRope && live) {
     ok = pos >= 0 && pos < a.max_positions;
     if (!ok && lane8 == 0) atomicOr(&g_kv8_status, MAC_B200_STATUS_BAD_REQUEST);
-    if (ok && !is_v)
-      rotate_row<kSplit, kVec>(a, row, a.cos_sin_cache + pos * a.cos_sin_stride0, lane8, x);
+    if (ok) rotate_row<kSplit, kVec>(a, row, a.cos_sin_cache + pos * a.cos_sin_stride0, lane8, x);
   }
   if (is_q && ok) {
     __nv_bfloat16* post = static_cast<__nv_bfloat16*>(a.q_post) + (n * a.Hq + h) * 128;
@@ -165,9 +167,9 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_write_kernel(const MacB200Qua
                      pack_bf16(x[g * 8 + 4], x[g * 8 + 5]), pack_bf16(x[g * 8 + 6], x[g * 8 + 7]));
   }
   const bool write = ok && !is_q && loc >= 0 && loc < a.kv_pool_tokens;
-  const int64_t at = (write ? loc : 0) * a.Hkv + h;
-  hold_row<kSplit>(x, lane8, static_cast<uint8_t*>(is_v ? a.v_pool : a.k_pool) + at * 128,
-                   (is_v ? a.v_exp : a.k_exp) + at, write);
+  const int64_t at = (write ? loc : 0) * a.Hkv + (write ? h : 0);
+  hold_row<kSplit>(x, lane8, static_cast<uint8_t*>(a.k_pool) + at * 128, a.k_exp + at, write);
+  hold_row<kSplit>(y, lane8, static_cast<uint8_t*>(a.v_pool) + at * 128, a.v_exp + at, write);
 }
 
 // One task = one (row, K or V, head): 16 codes a lane in one load, 16 bf16 out in two stores.
@@ -246,7 +248,7 @@ extern "C" int mac_b200_quantize_kv_e4m3(const MacB200QuantizeKvArgs* args, void
               "invalid rotary_dim");
   MAC_REQUIRE(!rope || on16(a.q_post), "q_post must be 16-byte aligned");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  const int64_t heads = 2 * static_cast<int64_t>(a.Hkv) + (rope ? a.Hq : 0);
+  const int64_t heads = static_cast<int64_t>(a.Hkv) + (rope ? a.Hq : 0);
   const unsigned blocks = blocks_for(a.N * heads);
   MAC_REQUIRE(blocks > 0, "quantize problem too large");
   const bool vec = on16(a.k) && on16(a.v) && a.k_stride0 % 8 == 0 && a.v_stride0 % 8 == 0;
