@@ -37,14 +37,16 @@ extern "C" {
  * A row that attends nothing (p < 0, window 0) gets out = 0, lse = -inf.  A
  * value that a row does not attend does not reach it, whatever it holds.
  *
- * Rows of q outside [offsets[0], offsets[B]) are neither read nor written in
- * out / lse.  All lengths are read on the device; nothing about a call has to
+ * Rows of q outside [offsets[0], offsets[B]) reach nothing and are not written
+ * in out / lse.  q and out must not share memory.  All lengths are read on the device; nothing about a call has to
  * change between replays of a captured graph but the contents of its tensors.
  *
  * What cannot be run sets MAC_B200_STATUS_BAD_REQUEST (mac_b200_query_status):
  * a request whose offsets are not inside [0, q_rows] or decrease is left out;
  * one whose req_id or length is outside the page table gets empty rows; a
- * page-table entry outside the pool counts as a row of zeros.
+ * page-table entry outside the pool counts as a row of zeros.  Waits inside the
+ * kernel are bounded (about two seconds); one that runs out ends the call with
+ * MAC_B200_STATUS_COPY_TIMEOUT, and its out and lse are not valid.
  */
 typedef struct MacB200ChunkArgs {
   int32_t B;                   /* requests                                                  */
@@ -62,7 +64,8 @@ typedef struct MacB200ChunkArgs {
   const void* q;               /* [q_rows,Hq,128] bf16, heads contiguous, 16-byte aligned   */
   const void* k;               /* pool: [kv_tokens,Hkv,128] bf16 or e4m3, 16-byte aligned   */
   const void* v;
-  const uint8_t* k_exp;        /* [kv_tokens,Hkv] exponent bytes (e4m3 pool), else NULL     */
+  const uint8_t* k_exp;        /* [kv_tokens,Hkv] exponent bytes (e4m3 pool), else NULL; read
+                                  in aligned blocks of 16 bytes, nothing behind the end     */
   const uint8_t* v_exp;
   const int32_t* req_to_token; /* [rows,stride] logical position -> pool row                */
   const int32_t* req_ids;      /* [B]                                                       */
@@ -71,8 +74,8 @@ typedef struct MacB200ChunkArgs {
   void* out;                   /* [q_rows,Hq,128] bf16, 16-byte aligned                     */
   float* lse;                  /* [q_rows,Hq] f32 natural log, or NULL                      */
   void* workspace;             /* mac_b200_chunk_attention_workspace_bytes() bytes, 16-byte
-                                  aligned, zeroed once when it is made; calls that may run at
-                                  the same time need one each                               */
+                                  aligned, whatever it holds; calls that may run at the same
+                                  time need one each                                        */
 } MacB200ChunkArgs;
 
 /* Chunk attention over a bf16 pool / over an e4m3 pool. */
@@ -92,7 +95,7 @@ int mac_b200_chunk_attention_workspace_bytes(int64_t* bytes);
  *
  * Rows of cache_locs outside [0, kv_pool_tokens) are not written to the pool
  * (padding).  Entries inside have to be distinct: a pool row named twice holds
- * bytes of either.  A position outside [0, max_positions) sets
+ * bytes of either.  q_post must not share memory with q, k or v.  A position outside [0, max_positions) sets
  * MAC_B200_STATUS_BAD_REQUEST; its token is neither rotated nor written.
  */
 typedef struct MacB200QuantizeKvArgs {

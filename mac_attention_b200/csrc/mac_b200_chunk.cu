@@ -1343,6 +1343,9 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
               "q row stride must be a multiple of 8 and at least Hq*128");
   MAC_REQUIRE(on16(a.q) && on16(a.k) && on16(a.v) && on16(a.out) && on16(a.workspace),
               "chunk tensors must be 16-byte aligned");
+  const int64_t out_bytes = a.q_rows * static_cast<int64_t>(a.Hq) * 256;
+  MAC_REQUIRE(!byte_ranges_meet(a.q, (a.q_rows - 1) * a.q_stride0 * 2 + a.Hq * int64_t{256}, a.out, out_bytes),
+              "q and out must not share memory");
   int device = 0;
   MAC_CUDA(cudaGetDevice(&device));
   const int sms = device_sm_count(device);

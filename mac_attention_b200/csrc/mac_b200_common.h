@@ -40,6 +40,12 @@ int take_kv8_status(unsigned* bits);
 int launch_prefill_sink_exclusive_tc(const ::MacB200PrefillBuildArgs& a, int sms, cudaStream_t stream,
                                      bool* launched);
 
+// Whether [a, a + a_bytes) and [b, b + b_bytes) have a byte in common.
+inline bool byte_ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x <= y ? y - x < static_cast<uintptr_t>(a_bytes) : x - y < static_cast<uintptr_t>(b_bytes);
+}
+
 // Multiprocessor count of a device, looked up once per device.
 int device_sm_count(int device);
 

@@ -247,6 +247,13 @@ extern "C" int mac_b200_quantize_kv_e4m3(const MacB200QuantizeKvArgs* args, void
   MAC_REQUIRE(!rope || (a.rotary_dim > 0 && a.rotary_dim <= 128 && a.rotary_dim % 2 == 0),
               "invalid rotary_dim");
   MAC_REQUIRE(!rope || on16(a.q_post), "q_post must be 16-byte aligned");
+  if (rope) {                                        // rows are read by other threads than those that write them
+    const int64_t last = a.N - 1, post_bytes = a.N * a.Hq * 256;
+    MAC_REQUIRE(!byte_ranges_meet(a.q, (last * a.q_stride0 + a.Hq * int64_t{128}) * 2, a.q_post, post_bytes) &&
+                    !byte_ranges_meet(a.k, (last * a.k_stride0 + a.Hkv * int64_t{128}) * 2, a.q_post, post_bytes) &&
+                    !byte_ranges_meet(a.v, (last * a.v_stride0 + a.Hkv * int64_t{128}) * 2, a.q_post, post_bytes),
+                "q_post must not share memory with q, k or v");
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const int64_t heads = static_cast<int64_t>(a.Hkv) + (rope ? a.Hq : 0);
   const unsigned blocks = blocks_for(a.N * heads);

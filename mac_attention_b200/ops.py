@@ -444,8 +444,8 @@ def mac_chunk_attention_bf16(q, k_buffer, v_buffer, req_to_token, req_ids, offse
     is free) are the last ``n`` of the ``kv_lens[b]`` tokens that ``req_to_token[req_ids[b]]``
     lists, already written to ``k_buffer`` / ``v_buffer`` ``[T,Hkv,128]``; ``Hq / Hkv`` is 1 to
     16.  The row at position ``p`` attends ``[max(0, p + 1 - window), p]`` (``window=None``:
-    all of ``[0, p]``).  ``out`` ``[rows,Hq,128]`` bf16 gets the result, ``lse`` ``[rows,Hq]``
-    (or ``None``) the natural-log LSE; a row that attends nothing gets 0 and ``-inf``, rows
+    all of ``[0, p]``).  ``out`` ``[rows,Hq,128]`` bf16 gets the result (not in ``q``'s memory), ``lse``
+    ``[rows,Hq]`` (or ``None``) the natural-log LSE; a row that attends nothing gets 0 and ``-inf``, rows
     outside ``[offsets[0], offsets[B])`` are left as they are.  ``window=None`` and
     ``window=semantic_pos_ahead`` give the full-prefix and the band state of
     :func:`mac_prefill_downdate_update_cache`.  Prompt chunks, drafted tokens and single
@@ -487,7 +487,8 @@ def mac_decode_rope_quantize_kv_e4m3(q, k, v, q_post, k_pool, v_pool, k_exp, v_e
     ``q`` ``[N, Hq*128]``, the pool rows ``cache_locs`` get the rotated ``k`` and ``v`` as
     :func:`mac_quantize_kv_e4m3` holds them (``k`` is rotated in fp32 and rounded once, to
     e4m3).  Counterpart of :func:`mac_decode_rope_preserve_q_bf16` for the 8-bit pool, with the
-    difference that ``q``, ``k``, ``v`` stay as they are: ``q`` itself is the pre-RoPE query.
+    difference that ``q``, ``k``, ``v`` stay as they are (``q_post`` must not share memory with
+    them): ``q`` itself is the pre-RoPE query.
     A token whose position lies outside ``cos_sin_cache`` is skipped and reported by
     :func:`query_status`."""
     _raise_on_failure(_load_shim().rope_quantize_kv(q, k, v, q_post, k_pool, v_pool, k_exp, v_exp, cos_sin_cache,

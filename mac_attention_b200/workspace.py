@@ -72,11 +72,10 @@ def make_decision_workspace(batch, hq, hkv, capacity, match_tile_slots, *, devic
 
 
 def make_chunk_attention_workspace(device="cuda"):
-    """The scratch of ``mac_chunk_attention_bf16`` / ``_e4m3``: split results and arrival
-    counters, whatever the sizes of the calls.  Its size depends on the device alone; it is
-    zeroed here once and every call leaves its counters at zero.  Calls that may overlap on
-    the device (two streams, two graphs replayed side by side) need one each; calls in order
-    share one."""
+    """The scratch of ``mac_chunk_attention_bf16`` / ``_e4m3``: the results of work that was
+    split, whatever the sizes of the calls.  Its size depends on the device alone and nothing in
+    it outlives a call.  Calls that may overlap on the device (two streams, two graphs replayed
+    side by side) need one each; calls in order share one."""
     import ctypes as C
 
     from . import _abi
@@ -87,7 +86,7 @@ def make_chunk_attention_workspace(device="cuda"):
     n = C.c_int64(0)
     with torch.cuda.device(dev):
         _abi.check(_abi.load_library().mac_b200_chunk_attention_workspace_bytes(C.byref(n)))
-        return torch.zeros(n.value, dtype=torch.uint8, device=dev)
+        return torch.empty(n.value, dtype=torch.uint8, device=dev)
 
 
 def make_quantized_pool(tokens, hkv, *, device="cuda"):

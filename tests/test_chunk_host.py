@@ -121,6 +121,18 @@ def test_quantize_refusals(lib, change, text):
     assert text in lib.mac_b200_last_error()
 
 
+def test_results_that_share_memory_with_their_inputs_are_refused(lib):
+    """Rows are read by other threads than those that write them: an overlap would race."""
+    q, held = 1 << 20, 4 * 8 * 256                         # four rows of eight heads
+    for out in (q, q + 2048, q + held - 16, q - held + 16):
+        assert lib.mac_b200_chunk_attention_bf16(C.byref(_chunk(q=q, out=out)), None) == -1
+        assert b"share memory" in lib.mac_b200_last_error()
+    for change in (dict(), dict(q=1 << 20, v=1 << 21), dict(k=1 << 20, v=1 << 21), dict(k=1 << 20, q=1 << 21)):
+        a = _quant(q_stride0=1024, k_stride0=256, v_stride0=256, **change)
+        assert lib.mac_b200_quantize_kv_e4m3(C.byref(a), None) == -1
+        assert b"q_post must not share memory" in lib.mac_b200_last_error()
+
+
 def _dequant(**change):
     a = _abi.MacB200DequantizeKvArgs()
     a.N, a.Hkv, a.D, a.src_tokens, a.dst_tokens = 2, 2, 128, 64, 64
