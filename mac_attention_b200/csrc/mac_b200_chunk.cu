@@ -22,7 +22,7 @@
 //                    maximum and sum in fp32, bf16 weights back over the scores, results out
 //   warps 0, 1       issue the streams' products: S = Q K^T from shared memory, O += P V with P from
 //                    tensor memory and V from the rows as they lie in the pool (keys x dims)
-//   warps 4-7 (-11)  fetch K/V rows by the page table into the swizzled operand layout (cp.async; the
+//   warps 4-7 (-15)  fetch K/V rows by the page table into the swizzled operand layout (cp.async; the
 //                    8-bit pool's rows by way of a raw buffer, widened to bf16)
 //   warp 2           works out the units of this CTA's part, fetches the query tiles
 // A stream goes in steps of 64 keys with two score buffers, so the products of the next step run
@@ -33,8 +33,9 @@
 //
 // Measured (B200: 6564 GB/s copied, 1675 TFLOP/s of a bf16 product):
 //   decode, 16 requests x 32768 tokens, 32 / 8 heads: 363 us, 0.87 of the copy rate (row fetches in
-//     flight bound it); the 8-bit pool 430 us, 0.37: the loading warps' instructions (widening,
-//     fetching and asking for rows, 2000 cycles a 16 KB position of two warps a scheduler)
+//     flight bound it); the 8-bit pool 375 us, 0.42: no one part bounds it (without
+//     the widening's stores 0.92 of the time, without the row fetches 0.96, without the softmax 0.93),
+//     the chain through three ring positions does
 //   prompt, 4096 tokens behind 28672 cached, 32 / 8 heads: 2.36 ms, 875 TFLOP/s; 2 x 1024 tokens of
 //     8192 over the 8-bit pool 571 us, 815 TFLOP/s.  Without the softmax's arithmetic such a call
 //     still takes 0.85 of its time: a product of 128 x 64 from shared memory is bound by the reads
@@ -114,7 +115,7 @@ struct Control {
   uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_done[2][2];
   uint64_t item_full[kItems], item_empty[kItems], join;
   Item items[kItems];
-  long long scan[20];      // a word a warp
+  long long scan[24];      // a word a warp
   long long start_pos;     // where request start_b begins on the line
   int start_b;
   uint32_t tmem;
@@ -125,27 +126,34 @@ struct Control {
 // Shared memory: two query tiles, the ring of K/V blocks, for the 8-bit pool the raw rows on their
 // way (each thread of the loading warps reads back what it fetched itself), the control words.
 // Registers a thread after the warpgroups have traded theirs:
-//   bf16: 128 * 64 + 128 * 160 + 256 * 144 = 512 * 128,  e4m3: 128 * 64 + 256 * 72 + 256 * 136 = 640 * 96
+//   bf16: 128 * 64 + 128 * 160 + 256 * 144 = 512 * 128,  e4m3: 128 * 64 + 384 * 48 + 256 * 128 <= 768 * 80
 constexpr int kSmemQ = 0;
 constexpr int kSmemKv = 2 * kTileBytes;
-constexpr int kRawSlots = 3;
 template <bool kE4m3>
 struct Layout {
-  static constexpr int kLoadWarps = kE4m3 ? 8 : 4;
+  static constexpr int kLoadWarps = kE4m3 ? 12 : 4;
+  static constexpr int kWarpRows = 32;                   // rows of a block that a loading warp fetches
   static constexpr int kSoftmaxWarp = kLoadWarp + kLoadWarps;
   static constexpr int kThreads = 32 * (kSoftmaxWarp + kSoftmaxWarps);
-  static constexpr int kLaunchRegs = kE4m3 ? 96 : 128, kControlRegs = 64;
-  static constexpr int kLoadRegs = kE4m3 ? 72 : 160, kSoftmaxRegs = kE4m3 ? 136 : 144;
-  static constexpr int kWarpRows = kBlk / kLoadWarps;    // rows of a block that a loading warp fetches
+  static constexpr int kLaunchRegs = kE4m3 ? 80 : 128, kControlRegs = 64;
+  static constexpr int kLoadRegs = kE4m3 ? 48 : 160, kSoftmaxRegs = kE4m3 ? 128 : 144;
   static constexpr int kStages = kE4m3 ? 3 : kMaxStages;
   static constexpr int kRawRows = kWarpRows * 128;       // of a warp and a ring position
   // with the 16 bytes around each row's exponent, and the table's entries of three positions later
   static constexpr int kRawExps = kRawRows, kRawEntries = kRawExps + kWarpRows * 16;
   static constexpr int kRawBytes = kRawEntries + kWarpRows * 4;
   static constexpr int kRaw = kSmemKv + kStages * kTileBytes;
-  static constexpr int kControl = kRaw + (kE4m3 ? kRawSlots * kLoadWarps * kRawBytes : 0);
+  static constexpr int kControl = kRaw + (kE4m3 ? kLoadWarps * kRawBytes : 0);
   static constexpr int kBytes = kControl + static_cast<int>(sizeof(Control));
 };
+template <typename L>
+constexpr bool registers_suffice() {
+  return 128 * L::kControlRegs + 32 * L::kLoadWarps * L::kLoadRegs + 32 * kSoftmaxWarps * L::kSoftmaxRegs <=
+         L::kThreads * L::kLaunchRegs;
+}
+static_assert(registers_suffice<Layout<false>>() && registers_suffice<Layout<true>>(),
+              "warps that ask for more registers than the CTA was launched with wait for ever");
+static_assert(Layout<true>::kLoadWarps == 4 * Layout<true>::kStages, "a group of four warps a ring position");
 static_assert(Layout<false>::kBytes <= 232448 && Layout<true>::kBytes <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -516,7 +524,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   // ---- barriers, tensor memory
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&ctl.kv_full[i], kE4m3 ? kLoadWarps : kLoadWarps * 32);
+      mbar_init(&ctl.kv_full[i], kE4m3 ? 4 : kLoadWarps * 32);
       mbar_init(&ctl.kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
@@ -553,13 +561,17 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kLoadRegs));
     else
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kLoadRegs));
-    const int part = (warp - kLoadWarp) * L::kWarpRows;  // this warp's rows of a block
+    const int part = ((warp - kLoadWarp) & 3) * L::kWarpRows;   // this warp's rows of a block
+    const int group = (warp - kLoadWarp) >> 2;           // e4m3: of four warps, by ring position
+    int base = 0;                                        // e4m3: ring position of a unit's first block
     uint32_t st = 0, phase = 1;                          // of the ring position to fill next
     bool ok = true;
     // bf16: sixteen lanes a row, straight into the swizzled operand layout (cp.async).
-    // e4m3: eight lanes a row, three ring positions ahead into a raw buffer (48 KB in flight; held in
-    // registers they were waited for all at once), then widened to bf16 with their scales on the way
-    // into the operand layout.  The widened rows are exact: from there on the two pools go the same way.
+    // e4m3: eight lanes a row, into a raw buffer ahead of time (48 KB of them; held in registers the rows
+    // were waited for all at once), then widened to bf16 with their scales on the way into the operand
+    // layout.  The widened rows are exact: from there on the two pools go the same way.  Four warps
+    // have a ring position to themselves, so three positions are widened at once (eight warps on one
+    // after the other: 430 us for the decode call above, 399 this way).
     constexpr int kLanes = kE4m3 ? 8 : 16, kPerLoad = 32 / kLanes;   // lanes a row, rows a load
     const int sub = lane / kLanes, c = lane % kLanes;    // row kPerLoad * j + sub of the part, 16 bytes of it
     const int64_t row_stride = static_cast<int64_t>(a.Hkv) * (kE4m3 ? 128 : 256);
@@ -572,8 +584,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       }
     }
     uint8_t* const wide = smem + kSmemKv + (c >> 2) * kHalfBytes + (part + sub) * 128;   // e4m3: the same, widened
-    uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * (kRawSlots * L::kRawBytes);
-    int bytes[kRawSlots];                                // which of its 16 bytes a row's exponent is
+    uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * L::kRawBytes;
     for (int it = 0; ok; ++it) {
       const int slot = it & (kItems - 1);
       ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
@@ -587,32 +598,31 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       const int32_t* table = a.req_to_token + static_cast<int64_t>(o.req) * a.req_to_token_stride;
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.item_empty[slot]);
-      // Key `lane` of this warp's part of the next ring position: the key, and what the table says of
-      // it.  Table entries are asked for ahead and looked at when they are needed.
-      struct Entry {
-        int key, row;
-        bool is_v;
-      };
-      int k_next = 0, v_next = 0;                        // blocks asked for; see ring_v()
-      auto entry_of = [&]() {
-        Entry e{khi, 0, false};
-        if (v_next == nblk) return e;
-        e.is_v = k_next == nblk || k_next > v_next + (dual ? 0 : 1);
-        e.key = first + (e.is_v ? v_next++ : k_next++) * kBlk + part + lane;
-        if (lane >= L::kWarpRows) e.key = khi;
-        if (!kE4m3 && e.key < khi) e.row = load_early(table + e.key);
-        return e;
-      };
-      // the pool row; -1: no key, or one outside the pool (reported): arrives as zeros
-      auto row_of = [&](const Entry& e) {
-        if (e.key >= khi) return -1;
-        if (e.row >= 0 && e.row < a.kv_tokens) return e.row;
-        atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
-        return -1;
-      };
-      // Entries are refilled where they were used: moved on to another one they would be waited for.
       const int n = 2 * nblk;
       if constexpr (!kE4m3) {
+        // Key `lane` of this warp's part of the next ring position: the key, and what the table says of
+        // it.  Table entries are asked for ahead and looked at when they are needed.
+        struct Entry {
+          int key, row;
+          bool is_v;
+        };
+        int k_next = 0, v_next = 0;                        // blocks asked for; see ring_v()
+        auto entry_of = [&]() {
+          Entry e{khi, 0, false};
+          if (v_next == nblk) return e;
+          e.is_v = k_next == nblk || k_next > v_next + (dual ? 0 : 1);
+          e.key = first + (e.is_v ? v_next++ : k_next++) * kBlk + part + lane;
+          if (e.key < khi) e.row = load_early(table + e.key);
+          return e;
+        };
+        // the pool row; -1: no key, or one outside the pool (reported): arrives as zeros
+        auto row_of = [&](const Entry& e) {
+          if (e.key >= khi) return -1;
+          if (e.row >= 0 && e.row < a.kv_tokens) return e.row;
+          atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+          return -1;
+        };
+        // Entries are refilled where they were used: moved on to another one they would be waited for.
         Entry e[2] = {entry_of(), entry_of()};
         for (int i0 = 0; i0 < n && ok; i0 += 2) {
 #pragma unroll
@@ -634,91 +644,110 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           }
         }
       } else {
-        auto fetch = [&](const Entry& e, int i) {
-          const int row = row_of(e);
-          uint8_t* const at_raw = raw + i * L::kRawBytes;
-          const uint8_t* exps = (e.is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + kh;
-          bytes[i] = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 15u);
-          const uint8_t* const end = (e.is_v ? a.v_exp : a.k_exp) + a.kv_tokens * a.Hkv;
+        // This group's positions of the unit are i0, i0 + 3, ...: those of its ring position.
+        const int i0 = (group + kStages - base) % kStages;
+        base = (base + n) % kStages;
+        // the key of this lane's row in local position i (see ring_v()); khi: none
+        auto key_of = [&](int i, bool& is_v) {
+          is_v = dual ? (i & 1) != 0 : i == n - 1 || (i > 0 && (i & 1) == 0);
+          const int blk = dual ? i >> 1 : is_v ? (i == n - 1 ? nblk : i >> 1) - 1 : (i + 1) >> 1;
+          return i < n ? first + blk * kBlk + part + lane : khi;
+        };
+        auto ask = [&](int i) {
+          bool is_v;
+          const int key = key_of(i, is_v);
+          if (key < khi) cp_async4(smem_u32(raw + L::kRawEntries + lane * 4), table + key, 4);
+        };
+        int row = 0, bytes = 0;                          // of position i: the pool row of this lane's key, its exponent's place
+        bool is_v = false;
+        auto asked = [&](int i) {
+          const int key = key_of(i, is_v);
+          row = -1;
+          if (key < khi) {
+            row = *reinterpret_cast<const int*>(raw + L::kRawEntries + lane * 4);
+            if (row < 0 || row >= a.kv_tokens) {
+              row = -1;
+              atomicOr(&g_chunk_status, MAC_B200_STATUS_BAD_REQUEST);
+            }
+          }
+        };
+        auto fetch_exps = [&]() {
+          const uint8_t* exps = (is_v ? a.v_exp : a.k_exp) + static_cast<int64_t>(max(row, 0)) * a.Hkv + kh;
+          bytes = static_cast<int>(reinterpret_cast<uintptr_t>(exps) & 15u);
+          const uint8_t* const end = (is_v ? a.v_exp : a.k_exp) + a.kv_tokens * a.Hkv;
           // 16-byte copies pass the L1 cache by; single words would each hold a line of the little that
           // this much shared memory leaves of it, and wait for one
-          if (lane < L::kWarpRows)
-            cp_async16(smem_u32(at_raw + L::kRawExps + lane * 16), exps - bytes[i],
-                       row < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), end - (exps - bytes[i]))));
-          const uint8_t* src = static_cast<const uint8_t*>(e.is_v ? a.v : a.k) + col;
+          cp_async16(smem_u32(raw + L::kRawExps + lane * 16), exps - bytes,
+                     row < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), end - (exps - bytes))));
+        };
+        auto fetch_half = [&](int half) {
+          const uint8_t* src = static_cast<const uint8_t*>(is_v ? a.v : a.k) + col;
 #pragma unroll
-          for (int j = 0; j < L::kWarpRows / 4; ++j) {
-            const int tok = __shfl_sync(0xffffffffu, row, 4 * j + sub);
-            cp_async16(smem_u32(at_raw + j * 512 + lane * 16), src + max(tok, 0) * row_stride, tok < 0 ? 0 : 16);
+          for (int j = 0; j < 4; ++j) {
+            const int tok = __shfl_sync(0xffffffffu, row, half * 16 + 4 * j + sub);
+            cp_async16(smem_u32(raw + half * 2048 + j * 512 + lane * 16), src + max(tok, 0) * row_stride,
+                       tok < 0 ? 0 : 16);
           }
         };
         // Lanes of a row's second half widen and store their two chunks in the other order: no two lanes
         // of a row store to the same bank.
         const int flip = c >= 4 ? 1 : 0;
         const int c0 = 2 * (c & 3) + flip;
-        auto store = [&](int i) {
-          ok = ok && mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) return;
-          const uint8_t* const at_raw = raw + i * L::kRawBytes;
-          const uint32_t scale_own = scale_pair(at_raw[L::kRawExps + (lane % L::kWarpRows) * 16 + bytes[i]]);
+        auto store_half = [&](int half, uint32_t scale_own) {
           // everything is read before anything is stored: the compiler keeps reads behind stores that it
           // cannot tell apart from them
-          uint2 codes[L::kWarpRows / 4][2];
-          uint32_t scale_row[L::kWarpRows / 4];
+          uint2 codes[4][2];
+          uint32_t scale_row[4];
 #pragma unroll
-          for (int j = 0; j < L::kWarpRows / 4; ++j) {
-            codes[j][0] = *reinterpret_cast<const uint2*>(at_raw + j * 512 + lane * 16 + flip * 8);
-            codes[j][1] = *reinterpret_cast<const uint2*>(at_raw + j * 512 + lane * 16 + (flip ^ 1) * 8);
-            scale_row[j] = __shfl_sync(0xffffffffu, scale_own, 4 * j + sub);
+          for (int j = 0; j < 4; ++j) {
+            codes[j][0] = *reinterpret_cast<const uint2*>(raw + half * 2048 + j * 512 + lane * 16 + flip * 8);
+            codes[j][1] = *reinterpret_cast<const uint2*>(raw + half * 2048 + j * 512 + lane * 16 + (flip ^ 1) * 8);
+            scale_row[j] = __shfl_sync(0xffffffffu, scale_own, half * 16 + 4 * j + sub);
           }
 #pragma unroll
-          for (int j = 0; j < L::kWarpRows / 4; ++j) {
-            uint8_t* row = wide + st * kTileBytes + j * 512;
-            const int key = (part + 4 * j + sub) & 7;    // the swizzle
-            *reinterpret_cast<uint4*>(row + ((c0 ^ key) << 4)) = widen8(codes[j][0], scale_row[j]);
-            *reinterpret_cast<uint4*>(row + ((c0 ^ 1 ^ key) << 4)) = widen8(codes[j][1], scale_row[j]);
+          for (int j = 0; j < 4; ++j) {
+            uint8_t* to_row = wide + group * kTileBytes + half * 2048 + j * 512;
+            const int key = (4 * j + sub) & 7;           // the swizzle
+            *reinterpret_cast<uint4*>(to_row + ((c0 ^ key) << 4)) = widen8(codes[j][0], scale_row[j]);
+            *reinterpret_cast<uint4*>(to_row + ((c0 ^ 1 ^ key) << 4)) = widen8(codes[j][1], scale_row[j]);
           }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.kv_full[st]);
-          if (++st == kStages) st = 0, phase ^= 1u;
         };
-        // Table entries come by cp.async too: a load into a register shares its scoreboard with the
-        // loads of the widening, which would wait for it.
-        Entry e[kRawSlots];
-        auto ask = [&](int i) {
-          e[i] = entry_of();
-          if (e[i].key < khi)
-            cp_async4(smem_u32(raw + i * L::kRawBytes + L::kRawEntries + lane * 4), table + e[i].key, 4);
-        };
-        auto asked = [&](int i) {
-          if (e[i].key < khi)
-            e[i].row = *reinterpret_cast<const int*>(raw + i * L::kRawBytes + L::kRawEntries + lane * 4);
-        };
-#pragma unroll
-        for (int i = 0; i < kRawSlots; ++i) ask(i);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < kRawSlots; ++i) {
-          asked(i);
-          if (i < n) fetch(e[i], i);
-          ask(i);
+        // A group of copies a half, empty ones too.  The first half's holds the exponents of both and the
+        // entries of the group's next position.
+        if (i0 < n) {
+          ask(i0);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          asked(i0);
+          fetch_exps();
+          fetch_half(0);
+          ask(i0 + kStages);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          fetch_half(1);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        for (int i0 = 0; i0 < n && ok; i0 += kRawSlots) {
-#pragma unroll
-          for (int i = 0; i < kRawSlots; ++i) {
-            if (i0 + i >= n || !ok) break;
-            // one group a position, empty ones too: all but the last two have landed, this position's
-            // rows and the entries of the one three later among them
-            asm volatile("cp.async.wait_group 2;" ::: "memory");
-            asked(i);
-            store(i);
-            if (i0 + i + kRawSlots < n) fetch(e[i], i);
-            ask(i);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+        for (int i = i0; i < n; i += kStages) {
+          ok = mbar_wait(&ctl.kv_empty[group], phase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          phase ^= 1u;
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          const uint32_t scale_own = scale_pair(raw[L::kRawExps + lane * 16 + bytes]);
+          store_half(0, scale_own);
+          const bool more = i + kStages < n;
+          asked(i + kStages);                            // from here on row, is_v and bytes are the next position's
+          if (more) {
+            fetch_exps();
+            fetch_half(0);
+            ask(i + 2 * kStages);
           }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          store_half(1, scale_own);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.kv_full[group]);
+          if (more) fetch_half(1);
+          asm volatile("cp.async.commit_group;" ::: "memory");
         }
       }
     }
@@ -881,49 +910,60 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         // takes score buffer t & 1, and its weights lie where its scores were.
         const int steps = 2 * n - (n > 0 && keys - (dual ? n - 1 : 2 * (n - 1) + s) * kBlk <= kHalf ? 1 : 0);
         int st_k = 0, st_v = 0;
-        for (int i = 0; i < (steps > 0 ? steps + 2 : 0); ++i) {
+        const uint32_t t0 = t;
+        auto pv = [&](int i) {                           // O += P V of step i
+          if (!ok || i < 0 || i >= steps) return;
           const int h = i & 1;
-          if (i >= 2) {                                  // O += P V of step i - 2
-            const uint32_t b = t & 1;
-            if (h == 0) st_v = next_stage();
-            ok = ok && mbar_wait(&ctl.p_full[s][b], t >> 1, abort_flag);
+          const uint32_t b = t & 1;
+          if (h == 0) st_v = next_stage();
+          ok = ok && mbar_wait(&ctl.p_full[s][b], t >> 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          ++t;
+          fence_async_smem();
+          tc_fence_after();
+          const uint64_t dv = desc_v + uniform(st_v) * kDescTile + h * kDescHalf;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)                  // 16 keys each: two eight-row groups of V
+              mma_ts(t_o, t_s + b * kHalf + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4), i > 0 || k > 0);
+            mma_commit(&ctl.o_done[s][b]);
+            if (h == 1 || i == steps - 1) mma_commit(&ctl.kv_empty[st_v]);
+          }
+          __syncwarp();
+        };
+        auto qk = [&](int i) {                           // S = Q K^T of step i, into the buffer just emptied
+          if (!ok || i >= steps) return;
+          const int h = i & 1;
+          const uint32_t b = (t0 + i) & 1;
+          if (h == 0) {
+            st_k = next_stage();
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            ++t;
+            if (!ok) return;
             fence_async_smem();
-            tc_fence_after();
-            const uint64_t dv = desc_v + uniform(st_v) * kDescTile + h * kDescHalf;
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)                // 16 keys each: two eight-row groups of V
-                mma_ts(t_o, t_s + b * kHalf + k * 8, dv + static_cast<uint64_t>(k * 2048 >> 4), i > 2 || k > 0);
-              mma_commit(&ctl.o_done[s][b]);
-              if (h == 1 || i == steps + 1) mma_commit(&ctl.kv_empty[st_v]);
-            }
-            __syncwarp();
           }
-          if (i < steps) {                               // S = Q K^T of step i, into the buffer just emptied
-            const uint32_t b = (i < 2 ? t + i : t - 1) & 1;
-            if (h == 0) {
-              st_k = next_stage();
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              fence_async_smem();
-            }
-            tc_fence_after();
-            const uint64_t dk = desc_k + uniform(st_k) * kDescTile + h * kDescHalf;
-            if (elect_one()) {
+          tc_fence_after();
+          const uint64_t dk = desc_k + uniform(st_k) * kDescTile + h * kDescHalf;
+          if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
-                mma_ss(t_s + b * kHalf, dq + off, dk + off, k > 0);
-              }
-              mma_commit(&ctl.s_full[s][b]);
-              if (h == 1 || i == steps - 1) mma_commit(&ctl.kv_empty[st_k]);
-              if (i == steps - 1) mma_commit(&ctl.q_empty[buf]);
+            for (int k = 0; k < 8; ++k) {
+              const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4);
+              mma_ss(t_s + b * kHalf, dq + off, dk + off, k > 0);
             }
-            __syncwarp();
+            mma_commit(&ctl.s_full[s][b]);
+            if (h == 1 || i == steps - 1) mma_commit(&ctl.kv_empty[st_k]);
+            if (i == steps - 1) mma_commit(&ctl.q_empty[buf]);
           }
+          __syncwarp();
+        };
+        if (kE4m3 && !dual) {
+          // Where the ring is as short as three positions and the streams alternate, both products of a
+          // block's values come before the scores of the stream's next block: values that wait for the
+          // next keys before they are given back hold up the keys behind them.  (Decode of 16 x 32000
+          // tokens 375 us, 441 in the other order; five positions of bf16 gain nothing by it.)
+          for (int i = 0; ok && steps > 0 && i < steps + 2; i += 2) pv(i - 2), pv(i - 1), qk(i), qk(i + 1);
+        } else {
+          for (int i = 0; ok && steps > 0 && i < steps + 2; ++i) pv(i - 2), qk(i);
         }
         while (ok && at < 2 * nblk) {                    // the other stream's last positions
           ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
