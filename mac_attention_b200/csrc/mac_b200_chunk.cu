@@ -32,12 +32,12 @@
 // operand type); the sum of weights is taken before that rounding, in fp32.
 //
 // Measured (B200: 6564 GB/s copied, 1675 TFLOP/s of a bf16 product):
-//   decode, 16 requests x 32768 tokens, 32 / 8 heads: 363 us, 0.87 of the copy rate (row fetches in
-//     flight bound it); the 8-bit pool 375 us, 0.42: no one part bounds it (without
+//   decode, 16 requests x 32768 tokens, 32 / 8 heads: 323 us back to back, 0.98 of the copy rate (390
+//     with cold caches); the 8-bit pool 349 (392) us, 0.46 (0.41): no one part bounds it (without
 //     the widening's stores 0.92 of the time, without the row fetches 0.96, without the softmax 0.93),
-//     the chain through three ring positions does
-//   prompt, 4096 tokens behind 28672 cached, 32 / 8 heads: 2.36 ms, 875 TFLOP/s; 2 x 1024 tokens of
-//     8192 over the 8-bit pool 571 us, 815 TFLOP/s.  Without the softmax's arithmetic such a call
+//     the chain through the ring's few positions does
+//   prompt, 4096 tokens behind 28672 cached, 32 / 8 heads: 2.30 ms, 897 TFLOP/s; 2 x 1024 tokens of
+//     8192 over the 8-bit pool 555 us, 840 TFLOP/s.  Without the softmax's arithmetic such a call
 //     still takes 0.85 of its time: a product of 128 x 64 from shared memory is bound by the reads
 //     of its operands (412 cycles for 256 of arithmetic) and the hand-overs between the products
 //     and the softmax are not hidden entirely.  ncu: tensor cores 40 %, issue slots 44 %, exponentials
@@ -123,7 +123,7 @@ struct Control {
   float2 ml[2][kRows];     // a single unit's maxima and sums, by stream
 };
 
-// Shared memory: two query tiles, the ring of K/V blocks, for the 8-bit pool the raw rows on their
+// Shared memory: two query tiles, the ring of K/V blocks (with the second tile where it is not needed), for the 8-bit pool the raw rows on their
 // way (each thread of the loading warps reads back what it fetched itself), the control words.
 // Registers a thread after the warpgroups have traded theirs:
 //   bf16: 128 * 64 + 128 * 160 + 256 * 144 = 512 * 128,  e4m3: 128 * 64 + 384 * 48 + 256 * 128 <= 768 * 80
@@ -137,7 +137,7 @@ struct Layout {
   static constexpr int kThreads = 32 * (kSoftmaxWarp + kSoftmaxWarps);
   static constexpr int kLaunchRegs = kE4m3 ? 80 : 128, kControlRegs = 64;
   static constexpr int kLoadRegs = kE4m3 ? 48 : 160, kSoftmaxRegs = kE4m3 ? 128 : 144;
-  static constexpr int kStages = kE4m3 ? 3 : kMaxStages;
+  static constexpr int kStages = kE4m3 ? 3 : 5;
   static constexpr int kRawRows = kWarpRows * 128;       // of a warp and a ring position
   // with the 16 bytes around each row's exponent, and the table's entries of three positions later
   static constexpr int kRawExps = kRawRows, kRawEntries = kRawExps + kWarpRows * 16;
@@ -153,7 +153,6 @@ constexpr bool registers_suffice() {
 }
 static_assert(registers_suffice<Layout<false>>() && registers_suffice<Layout<true>>(),
               "warps that ask for more registers than the CTA was launched with wait for ever");
-static_assert(Layout<true>::kLoadWarps == 4 * Layout<true>::kStages, "a group of four warps a ring position");
 static_assert(Layout<false>::kBytes <= 232448 && Layout<true>::kBytes <= 232448, "shared memory of a CTA");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -472,6 +471,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   // the joining kernel may be set up from here on; it waits for this one's end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using L = Layout<kE4m3>;
+  constexpr int kGroups = kE4m3 ? L::kLoadWarps / 4 : 1;   // of loading warps, that take positions in turn
   constexpr int kStages = L::kStages, kThreads = L::kThreads, kLoadWarps = L::kLoadWarps;
   constexpr int kSoftmaxWarp = L::kSoftmaxWarp;
   Control& ctl = *reinterpret_cast<Control*>(smem + Layout<kE4m3>::kControl);
@@ -490,6 +490,10 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
                         ((b == b0 ? mine0 : load_request(a, b, blockIdx.x == 0)).n + tile_tokens - 1) / tile_tokens);
   // pairs of tiles once there are enough of them for every CTA
   const int span = scan_cta<kThreads>(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
+  // The 8-bit pool's ring is short.  Where every unit is of one tile the second query buffer, in front of
+  // it, joins it (decode 403 -> 392 us; a sixth position of bf16 gains nothing: 391 either way).
+  const int stages = kE4m3 && span == tile_tokens ? kStages + 1 : kStages;
+  uint8_t* const ring = smem + kSmemKv - (stages - kStages) * kTileBytes;
   long long units = 0;
   mine = 0;
   for (int b = b0; b < b1; ++b) {
@@ -523,7 +527,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
 
   // ---- barriers, tensor memory
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(&ctl.kv_full[i], kE4m3 ? 4 : kLoadWarps * 32);
       mbar_init(&ctl.kv_empty[i], 2);
     }
@@ -562,28 +566,29 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     else
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kLoadRegs));
     const int part = ((warp - kLoadWarp) & 3) * L::kWarpRows;   // this warp's rows of a block
-    const int group = (warp - kLoadWarp) >> 2;           // e4m3: of four warps, by ring position
-    int base = 0;                                        // e4m3: ring position of a unit's first block
+    const int group = (warp - kLoadWarp) >> 2;           // e4m3: of four warps, for every third position
     uint32_t st = 0, phase = 1;                          // of the ring position to fill next
+    int own = group;                                     // e4m3: the group's next position of the unit
+    if (kE4m3) st = group;
     bool ok = true;
     // bf16: sixteen lanes a row, straight into the swizzled operand layout (cp.async).
     // e4m3: eight lanes a row, into a raw buffer ahead of time (48 KB of them; held in registers the rows
     // were waited for all at once), then widened to bf16 with their scales on the way into the operand
     // layout.  The widened rows are exact: from there on the two pools go the same way.  Four warps
-    // have a ring position to themselves, so three positions are widened at once (eight warps on one
-    // after the other: 430 us for the decode call above, 399 this way).
-    constexpr int kLanes = kE4m3 ? 8 : 16, kPerLoad = 32 / kLanes;   // lanes a row, rows a load
-    const int sub = lane / kLanes, c = lane % kLanes;    // row kPerLoad * j + sub of the part, 16 bytes of it
+    // take every third position, so three are widened at once (eight warps on one after the other:
+    // 430 us for the decode call above, 398 this way).
+    constexpr int kLanes = kE4m3 ? 8 : 16;               // of a row
+    const int sub = lane / kLanes, c = lane % kLanes;    // row of a load, 16 bytes of it
     const int64_t row_stride = static_cast<int64_t>(a.Hkv) * (kE4m3 ? 128 : 256);
     uint32_t to[4];                                      // bf16: where this lane's chunk goes in rows 2i + sub
     if constexpr (!kE4m3) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = part + 2 * i + sub;
-        to[i] = smem_u32(smem + kSmemKv) + (c >> 3) * kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        to[i] = smem_u32(ring) + (c >> 3) * kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
       }
     }
-    uint8_t* const wide = smem + kSmemKv + (c >> 2) * kHalfBytes + (part + sub) * 128;   // e4m3: the same, widened
+    uint8_t* const wide = ring + (c >> 2) * kHalfBytes + (part + sub) * 128;   // e4m3: the same, widened
     uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * L::kRawBytes;
     for (int it = 0; ok; ++it) {
       const int slot = it & (kItems - 1);
@@ -640,13 +645,12 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
                          tok < 0 ? 0 : 16);
             }
             cp_async_arrive(&ctl.kv_full[st]);
-            if (++st == kStages) st = 0, phase ^= 1u;
+            if (++st == stages) st = 0, phase ^= 1u;
           }
         }
       } else {
-        // This group's positions of the unit are i0, i0 + 3, ...: those of its ring position.
-        const int i0 = (group + kStages - base) % kStages;
-        base = (base + n) % kStages;
+        // This group's positions of the unit are i0, i0 + 3, ...
+        const int i0 = own;
         // the key of this lane's row in local position i (see ring_v()); khi: none
         auto key_of = [&](int i, bool& is_v) {
           is_v = dual ? (i & 1) != 0 : i == n - 1 || (i > 0 && (i & 1) == 0);
@@ -706,7 +710,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            uint8_t* to_row = wide + group * kTileBytes + half * 2048 + j * 512;
+            uint8_t* to_row = wide + st * kTileBytes + half * 2048 + j * 512;
             const int key = (4 * j + sub) & 7;           // the swizzle
             *reinterpret_cast<uint4*>(to_row + ((c0 ^ key) << 4)) = widen8(codes[j][0], scale_row[j]);
             *reinterpret_cast<uint4*>(to_row + ((c0 ^ 1 ^ key) << 4)) = widen8(codes[j][1], scale_row[j]);
@@ -720,35 +724,38 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           asked(i0);
           fetch_exps();
           fetch_half(0);
-          ask(i0 + kStages);
+          ask(i0 + kGroups);
           asm volatile("cp.async.commit_group;" ::: "memory");
           fetch_half(1);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        for (int i = i0; i < n; i += kStages) {
-          ok = mbar_wait(&ctl.kv_empty[group], phase, abort_flag);
+        int i = i0;
+        for (; i < n; i += kGroups) {
+          ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          phase ^= 1u;
           asm volatile("cp.async.wait_group 1;" ::: "memory");
           const uint32_t scale_own = scale_pair(raw[L::kRawExps + lane * 16 + bytes]);
           store_half(0, scale_own);
-          const bool more = i + kStages < n;
-          asked(i + kStages);                            // from here on row, is_v and bytes are the next position's
+          const bool more = i + kGroups < n;
+          asked(i + kGroups);                            // from here on row, is_v and bytes are the next position's
           if (more) {
             fetch_exps();
             fetch_half(0);
-            ask(i + 2 * kStages);
+            ask(i + 2 * kGroups);
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
           asm volatile("cp.async.wait_group 1;" ::: "memory");
           store_half(1, scale_own);
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.kv_full[group]);
+          if (lane == 0) mbar_arrive(&ctl.kv_full[st]);
+          st += kGroups;
+          if (st >= static_cast<uint32_t>(stages)) st -= stages, phase ^= 1u;
           if (more) fetch_half(1);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
+        own = i - n;
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");   // nothing in flight when the CTA leaves
@@ -830,7 +837,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
               tma_load_3d(dst, &q_map, 0, head * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
               tma_load_3d(dst + kHalfBytes, &q_map, 64, head * G, tok0 + i * tile_tokens, &ctl.q_full[buf]);
             }
-            if (!dual) toggle ^= 1;
+            if (!dual && stages == kStages) toggle ^= 1;
           }
           ++it;
         }
@@ -859,8 +866,8 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       uint32_t q_phase[2] = {0u, 0u}, t = 0;             // t: steps of 64 keys so far
       uint32_t st = 0, phase = 0;                        // of the ring position to wait for next
       const uint64_t desc_q = operand_desc(smem_u32(smem + kSmemQ), 16);
-      const uint64_t desc_k = operand_desc(smem_u32(smem + kSmemKv), 16);
-      const uint64_t desc_v = operand_desc(smem_u32(smem + kSmemKv), kHalfBytes);
+      const uint64_t desc_k = operand_desc(smem_u32(ring), 16);
+      const uint64_t desc_v = operand_desc(smem_u32(ring), kHalfBytes);
       constexpr uint64_t kDescTile = kTileBytes >> 4, kDescHalf = (kHalf * 128) >> 4;
       bool ok = true;
       for (int it = 0; ok; ++it) {
@@ -900,7 +907,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
             }
             const int found = static_cast<int>(st);
             ++at;
-            if (++st == kStages) st = 0, phase ^= 1u;
+            if (++st == stages) st = 0, phase ^= 1u;
             if (mine) return found;
           }
           return -1;
@@ -960,7 +967,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           // Where the ring is as short as three positions and the streams alternate, both products of a
           // block's values come before the scores of the stream's next block: values that wait for the
           // next keys before they are given back hold up the keys behind them.  (Decode of 16 x 32000
-          // tokens 375 us, 441 in the other order; five positions of bf16 gain nothing by it.)
+          // tokens 370 us, 441 in the other order; five positions of bf16 gain nothing by it.)
           for (int i = 0; ok && steps > 0 && i < steps + 2; i += 2) pv(i - 2), pv(i - 1), qk(i), qk(i + 1);
         } else {
           for (int i = 0; ok && steps > 0 && i < steps + 2; ++i) pv(i - 2), qk(i);
@@ -969,7 +976,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
           if (lane == 0) mbar_arrive(&ctl.kv_empty[st]);
           ++at;
-          if (++st == kStages) st = 0, phase ^= 1u;
+          if (++st == stages) st = 0, phase ^= 1u;
         }
         ok = __all_sync(0xffffffffu, ok);
       }
@@ -1023,11 +1030,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           // A weight of zero does not silence an infinite or NaN value in the product.  Such values
           // of a block that some rows attend only in part are taken out here and put back, for the
           // rows that do attend them, when the unit ends.
-          const uint32_t vp = pos + ring_v(dual, blk, nblk), st = vp % kStages;
-          ok = mbar_wait(&ctl.kv_full[st], vp / kStages, abort_flag);
+          const uint32_t vp = pos + ring_v(dual, blk, nblk), st = vp % stages;
+          ok = mbar_wait(&ctl.kv_full[st], vp / stages, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          uint32_t* v = reinterpret_cast<uint32_t*>(smem + kSmemKv + st * kTileBytes);
+          uint32_t* v = reinterpret_cast<uint32_t*>(ring + st * kTileBytes);
           unsigned found = 0;
 #pragma unroll 4
           for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
