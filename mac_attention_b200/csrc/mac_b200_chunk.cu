@@ -40,8 +40,8 @@
 //     8192 over the 8-bit pool 555 us, 840 TFLOP/s.  Without the softmax's arithmetic such a call
 //     still takes 0.85 of its time: a product of 128 x 64 from shared memory is bound by the reads
 //     of its operands (412 cycles for 256 of arithmetic) and the hand-overs between the products
-//     and the softmax are not hidden entirely.  ncu (1024 tokens of 8192, 64 / 8 heads): tensor cores 46 %, issue
-//     slots 44 %, exponentials 46 % of the cycles.
+//     and the softmax are not hidden entirely.  ncu (1024 tokens of 8192, 64 / 8 heads): tensor cores
+//     46 %, issue slots 44 %, exponentials 46 % of the cycles.
 //   8 prompts of 2048 in a band of 1024: 596 us, 611 TFLOP/s (masked halves of blocks count as none)
 //   three requests of drafted tokens behind 1000: 22 us a call by itself; a single token 11 us, of
 //     which 3 are set-up (lengths, tensor memory) and 5 the chain of one block's steps
@@ -123,8 +123,9 @@ struct Control {
   float2 ml[2][kRows];     // a single unit's maxima and sums, by stream
 };
 
-// Shared memory: two query tiles, the ring of K/V blocks (with the second tile where it is not needed), for the 8-bit pool the raw rows on their
-// way (each thread of the loading warps reads back what it fetched itself), the control words.
+// Shared memory: two query tiles, the ring of K/V blocks (the 8-bit pool's with the second tile where it is
+// not needed), for the 8-bit pool the raw rows on their way (each thread of the loading warps reads back
+// what it fetched itself), the control words.
 // Registers a thread after the warpgroups have traded theirs:
 //   bf16: 128 * 64 + 128 * 160 + 256 * 144 = 512 * 128,  e4m3: 128 * 64 + 384 * 48 + 256 * 128 <= 768 * 80
 constexpr int kSmemQ = 0;
@@ -651,7 +652,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       } else {
         // This group's positions of the unit are i0, i0 + 3, ...
         const int i0 = own;
-        // the key of this lane's row in local position i (see ring_v()); khi: none
+        // the key of this lane's row in position i of the unit (see ring_v()); khi: none
         auto key_of = [&](int i, bool& is_v) {
           is_v = dual ? (i & 1) != 0 : i == n - 1 || (i > 0 && (i & 1) == 0);
           const int blk = dual ? i >> 1 : is_v ? (i == n - 1 ? nblk : i >> 1) - 1 : (i + 1) >> 1;
@@ -662,7 +663,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           const int key = key_of(i, is_v);
           if (key < khi) cp_async4(smem_u32(raw + L::kRawEntries + lane * 4), table + key, 4);
         };
-        int row = 0, bytes = 0;                          // of position i: the pool row of this lane's key, its exponent's place
+        int row = 0, bytes = 0;                          // of a position: this lane's pool row, its exponent's place
         bool is_v = false;
         auto asked = [&](int i) {
           const int key = key_of(i, is_v);

@@ -5,11 +5,12 @@
 // Eight lanes own a row of k and the row of v beside it, 16 values of each: a lane's four 16-byte
 // loads are issued before anything is computed (one row at a time: 45 us for the call below), a
 // row's maximum is three shuffles away, and the codes leave as one 16-byte store a lane (128 bytes
-// a row).  Measured on a B200 that copies 6564 GB/s: 32768 tokens of 8 heads written in 41 us (0.75
-// of the copy rate, the latency of a block's one round of loads), 100000 read back in 105 us
-// (0.89, memory); one to 1000 tokens 4.2 to 4.7 us, the launch.  Under the half-split rotation a lane owns dims [8l, 8l+8) and
-// [64+8l, 64+8l+8) instead, so both members of a pair are in one thread; its codes leave as two
-// 8-byte stores.  The row's exponent is found from the bits of its maximum, no logarithm.
+// a row).  Under the half-split rotation a lane owns dims [8l, 8l+8) and [64+8l, 64+8l+8) instead, so
+// both members of a pair are in one thread; its codes leave as two 8-byte stores.  The row's exponent
+// is found from the bits of its maximum, no logarithm.
+// Measured on a B200 that copies 6564 GB/s: 32768 tokens of 8 heads written in 41 us (0.75 of the copy
+// rate, the latency of a block's one round of loads), 100000 read back in 106 us (0.88, memory); one
+// to 1000 tokens 4.2 to 4.9 us, the launch.
 #include <cuda_bf16.h>
 
 #include "mac_b200_common.h"
