@@ -42,7 +42,7 @@
 //     of its operands (412 cycles for 256 of arithmetic) and the hand-overs between the products
 //     and the softmax are not hidden entirely.  ncu (1024 tokens of 8192, 64 / 8 heads): tensor cores
 //     46 %, issue slots 44 %, exponentials 46 % of the cycles.
-//   8 prompts of 2048 in a band of 1024: 596 us, 611 TFLOP/s (masked halves of blocks count as none)
+//   8 prompts of 2048 in a band of 1024: 576 us, 632 TFLOP/s (masked halves of blocks count as none)
 //   three requests of drafted tokens behind 1000: 22 us a call by itself; a single token 11 us, of
 //     which 3 are set-up (lengths, tensor memory) and 5 the chain of one block's steps
 // No gain, measured on the same calls: steps of 128 keys, one warp that issues for both streams,
@@ -297,6 +297,19 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+// 32 bytes: one store of a whole sector where the address allows it.  Every lane of a warp writes to a row
+// of its own, and half sectors cost the memory system as much as whole ones (8 prompts of 2048 in a
+// band of 1024: 576 us, 605 with 16-byte stores, 547 with none).
+__device__ __forceinline__ void store32(uint4* dst, const uint32_t (&w)[8], bool aligned32) {
+  if (aligned32) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 // the largest of three, NaN if any is NaN
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -990,6 +1003,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     const uint32_t t_s = tmem + s * 128 + t_lane, t_o = tmem + 256 + s * 128 + t_lane;
     const float scale = a.sm_scale * 1.4426950408889634f;
     const float slack = 8.f / scale;                     // scores may exceed the kept maximum by this
+    const bool whole_sectors = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u;
     char* const slots = static_cast<char*>(a.workspace) + kCutBytes;
     uint32_t t = 0, j_uses = 0, pos = 0;                 // t: steps of this stream so far
     bool ok = true;
@@ -1226,12 +1240,12 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           if (live && !cut) {
             uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + orow * 256 + c * 64);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
+            for (int i = 0; i < 2; ++i) {
+              uint32_t w[8];
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                w[j] = l == 0.f ? 0u : pack_bf16(v[i * 8 + 2 * j] * inv, v[i * 8 + 2 * j + 1] * inv);
-              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int j = 0; j < 8; ++j)
+                w[j] = l == 0.f ? 0u : pack_bf16(v[i * 16 + 2 * j] * inv, v[i * 16 + 2 * j + 1] * inv);
+              store32(dst + 2 * i, w, whole_sectors);
             }
           } else if (live) {
             float4* dst = reinterpret_cast<float4*>(part) + c * 8 * kSlotRows + prow;   // four dims of all rows

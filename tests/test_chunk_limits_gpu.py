@@ -139,6 +139,23 @@ def test_exponents_at_odd_addresses(ext, q8, shift, Hkv):
     assert ops.query_status() == 0
 
 
+@pytest.mark.parametrize("lens,kv", [([3, 70, 1], [50, 300, 129]), ([1], [3000]), ([400] * 40, [400] * 40)])
+def test_results_that_start_between_sectors(ext, lens, kv):
+    """out at an address that is a multiple of 16 bytes but not of 32, inside a larger array."""
+    t = make_chunk(lens, kv, 16, 2, seed=36)
+    n = t["q"].numel()
+    wide = torch.full((n + 32,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = wide[8:8 + n].view(t["q"].shape)
+    assert out.data_ptr() % 32 == 16
+    lse = torch.zeros(t["q"].shape[:2], device="cuda")
+    ws = mac.make_chunk_attention_workspace()
+    ext.mac_chunk_attention_bf16(t["q"], t["k"], t["v"], t["table"], t["ids"], t["offsets"], t["kv_lens"], out, lse, ws)
+    assert_chunk_close(out, lse, chunk_reference(t))
+    assert (wide[:8] == 7).all() and (wide[8 + n:] == 7).all()
+    other, other_lse = run(ext, t, ws)
+    assert torch.equal(out, other) and torch.equal(lse, other_lse) and ops.query_status() == 0
+
+
 def test_workspace_contents_do_not_matter(ext):
     t = make_chunk([1, 1, 150], [3000, 700, 2000], 8, 2, seed=33)
     ws = mac.make_chunk_attention_workspace()
