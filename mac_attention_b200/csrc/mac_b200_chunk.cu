@@ -298,19 +298,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 32 bytes: one store of a whole sector where the address allows it.  Every lane of a warp writes to a row
-// of its own, and half sectors cost the memory system as much as whole ones (8 prompts of 2048 in a
-// band of 1024: 576 us, 605 with 16-byte stores, 547 with none).
-__device__ __forceinline__ void store32(uint4* dst, const uint32_t (&w)[8], bool aligned32) {
-  if (aligned32) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-  } else {
-    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  }
-}
 // the largest of three, NaN if any is NaN
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;

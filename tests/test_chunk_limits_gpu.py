@@ -156,6 +156,20 @@ def test_results_that_start_between_sectors(ext, lens, kv):
     assert torch.equal(out, other) and torch.equal(lse, other_lse) and ops.query_status() == 0
 
 
+def test_rows_read_back_between_sectors(q8):
+    """Buffers at an address that is a multiple of 16 bytes but not of 32, inside a larger array."""
+    t = make_chunk([9], [200], 8, 2, seed=37)
+    (kp, vp, ke, ve), k, v = quantized(t)
+    n = k.numel()
+    wide = torch.full((2, n + 32), 7.0, dtype=torch.bfloat16, device="cuda")
+    bufs = [wide[i, 8 + 16 * i:8 + 16 * i + n].view(k.shape) for i in range(2)]
+    assert all(b.data_ptr() % 32 == 16 for b in bufs)
+    q8.mac_dequantize_kv_e4m3(kp, vp, ke, ve, torch.arange(k.shape[0], device="cuda"), *bufs)
+    for i, (b, want) in enumerate(zip(bufs, (k, v))):
+        assert torch.equal(b.view(torch.int16), want.view(torch.int16))
+        assert (wide[i, :8 + 16 * i] == 7).all() and (wide[i, 8 + 16 * i + n:] == 7).all()
+
+
 def test_workspace_contents_do_not_matter(ext):
     t = make_chunk([1, 1, 150], [3000, 700, 2000], 8, 2, seed=33)
     ws = mac.make_chunk_attention_workspace()
