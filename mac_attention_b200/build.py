@@ -20,6 +20,7 @@ SOURCES = ["mac_b200_api.cu", "mac_b200_prefill.cu", "mac_b200_decode.cu", "mac_
            "mac_b200_downdate.cu", "mac_b200_prefill_build.cu", "mac_b200_prefill_sink_tc.cu",
            "mac_b200_chunk.cu", "mac_b200_kv8.cu"]
 HEADERS = [CSRC / "mac_b200_common.h", CSRC / "mac_b200_state_math.cuh", CSRC / "mac_b200_kv8.cuh",
+           CSRC / "mac_b200_chunk_ring.h",
            PKG.parent / "include" / "mac_b200.h", PKG.parent / "include" / "mac_b200_chunk.h"]
 
 

@@ -55,6 +55,7 @@
 #include <climits>
 #include <cmath>
 
+#include "mac_b200_chunk_ring.h"
 #include "mac_b200_common.h"
 #include "mac_b200_kv8.cuh"
 
@@ -132,13 +133,13 @@ constexpr int kSmemQ = 0;
 constexpr int kSmemKv = 2 * kTileBytes;
 template <bool kE4m3>
 struct Layout {
-  static constexpr int kLoadWarps = kE4m3 ? 12 : 4;
+  static constexpr int kLoadWarps = 4 * RingShape<kE4m3>::kGroups;
   static constexpr int kWarpRows = 32;                   // rows of a block that a loading warp fetches
   static constexpr int kSoftmaxWarp = kLoadWarp + kLoadWarps;
   static constexpr int kThreads = 32 * (kSoftmaxWarp + kSoftmaxWarps);
   static constexpr int kLaunchRegs = kE4m3 ? 80 : 128, kControlRegs = 64;
   static constexpr int kLoadRegs = kE4m3 ? 48 : 160, kSoftmaxRegs = kE4m3 ? 128 : 144;
-  static constexpr int kStages = kE4m3 ? 3 : 5;
+  static constexpr int kStages = RingShape<kE4m3>::kStages;
   static constexpr int kRawRows = kWarpRows * 128;       // of a warp and a ring position
   // with the 16 bytes around each row's exponent, and the table's entries of three positions later
   static constexpr int kRawExps = kRawRows, kRawEntries = kRawExps + kWarpRows * 16;
@@ -472,7 +473,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   // the joining kernel may be set up from here on; it waits for this one's end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using L = Layout<kE4m3>;
-  constexpr int kGroups = kE4m3 ? L::kLoadWarps / 4 : 1;   // of loading warps, that take positions in turn
+  constexpr int kGroups = RingShape<kE4m3>::kGroups;     // of loading warps, that take positions in turn
   constexpr int kStages = L::kStages, kThreads = L::kThreads, kLoadWarps = L::kLoadWarps;
   constexpr int kSoftmaxWarp = L::kSoftmaxWarp;
   Control& ctl = *reinterpret_cast<Control*>(smem + Layout<kE4m3>::kControl);
@@ -493,7 +494,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
   const int span = scan_cta<kThreads>(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
   // The 8-bit pool's ring is short.  Where every unit is of one tile the second query buffer, in front of
   // it, joins it (decode 403 -> 392 us; a sixth position of bf16 gains nothing: 391 either way).
-  const int stages = kE4m3 && span == tile_tokens ? kStages + 1 : kStages;
+  const int stages = span == tile_tokens ? kStages + RingShape<kE4m3>::kSpare : kStages;
   uint8_t* const ring = smem + kSmemKv - (stages - kStages) * kTileBytes;
   long long units = 0;
   mine = 0;
@@ -732,7 +733,9 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         }
         int i = i0;
         for (; i < n; i += kGroups) {
-          ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
+          ok = wait_to_fill([&](bool filled) {
+            return mbar_wait(filled ? &ctl.kv_full[st] : &ctl.kv_empty[st], phase, abort_flag);
+          });
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           asm volatile("cp.async.wait_group 1;" ::: "memory");
