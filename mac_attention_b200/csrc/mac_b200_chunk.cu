@@ -182,8 +182,9 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 // Waits for the phase of the given parity.  False when the limit ran out here or in another warp of
-// the CTA: the caller leaves its loop.  Short on purpose: it stands at two dozen places, and what
-// the warps of a scheduler execute in turn has to stay in its instruction cache.
+// the CTA: the caller leaves its loop.  For one lane by itself, or where a vote follows.  Short on
+// purpose: it stands at two dozen places, and what the warps of a scheduler execute in turn has to stay
+// in its instruction cache.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned* abort_flag) {
   const uint32_t b = smem_u32(bar);
   if (mbar_try(b, parity & 1u)) return true;
@@ -196,6 +197,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
     }
   }
   return true;
+}
+// The same for a warp whose lanes go on together.  The limit can run out for one lane and not for the
+// next; lanes that then took different ways would meet each other's votes, and wait for ever.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
 }
 
 __device__ __forceinline__ void tc_fence_before() {
@@ -594,8 +600,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     uint8_t* const raw = smem + L::kRaw + (warp - kLoadWarp) * L::kRawBytes;
     for (int it = 0; ok; ++it) {
       const int slot = it & (kItems - 1);
-      ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&ctl.item_full[slot], it / kItems, abort_flag);
       if (!ok) break;
       const Item& o = ctl.items[slot];
       if (!o.valid) break;
@@ -634,8 +639,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         for (int i0 = 0; i0 < n && ok; i0 += 2) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {                  // n is even
-            ok = mbar_wait(&ctl.kv_empty[st], phase, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = warp_wait(&ctl.kv_empty[st], phase, abort_flag);
             if (!ok) break;
             const char* src = static_cast<const char*>(e[i].is_v ? a.v : a.k) + col;
             const int row = row_of(e[i]);
@@ -734,9 +738,8 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         int i = i0;
         for (; i < n; i += kGroups) {
           ok = wait_to_fill([&](bool filled) {
-            return mbar_wait(filled ? &ctl.kv_full[st] : &ctl.kv_empty[st], phase, abort_flag);
+            return warp_wait(filled ? &ctl.kv_full[st] : &ctl.kv_empty[st], phase, abort_flag);
           });
-          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           asm volatile("cp.async.wait_group 1;" ::: "memory");
           const uint32_t scale_own = scale_pair(raw[L::kRawExps + lane * 16 + bytes]);
@@ -876,8 +879,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       bool ok = true;
       for (int it = 0; ok; ++it) {
         const int slot = it & (kItems - 1);
-        ok = mbar_wait(&ctl.item_full[slot], it / kItems, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait(&ctl.item_full[slot], it / kItems, abort_flag);
         if (!ok) break;
         const Item& o = ctl.items[slot];
         if (!uniform(o.valid)) break;
@@ -894,7 +896,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         // tiles.
         for (int i = 0; i < 2; ++i)
           if (dual || i == qbuf) {
-            ok = ok && mbar_wait(&ctl.q_full[i], q_phase[i], abort_flag);
+            ok = ok && warp_wait(&ctl.q_full[i], q_phase[i], abort_flag);
             q_phase[i] ^= 1u;
             if ((i != buf || n == 0) && lane == 0) mbar_arrive(&ctl.q_empty[i]);
           }
@@ -902,7 +904,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
         // waits for the stream's next own position; its stage, or -1
         auto next_stage = [&]() {
           while (ok) {
-            ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
+            ok = warp_wait(&ctl.kv_full[st], phase, abort_flag);
             bool mine = true;
             if (!dual) {
               const bool is_v = k_next == nblk || k_next > v_next + 1;
@@ -927,8 +929,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           const int h = i & 1;
           const uint32_t b = t & 1;
           if (h == 0) st_v = next_stage();
-          ok = ok && mbar_wait(&ctl.p_full[s][b], t >> 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = ok && warp_wait(&ctl.p_full[s][b], t >> 1, abort_flag);
           if (!ok) return;
           ++t;
           fence_async_smem();
@@ -949,7 +950,6 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           const uint32_t b = (t0 + i) & 1;
           if (h == 0) {
             st_k = next_stage();
-            ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
             fence_async_smem();
           }
@@ -977,12 +977,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           for (int i = 0; ok && steps > 0 && i < steps + 2; ++i) pv(i - 2), qk(i);
         }
         while (ok && at < 2 * nblk) {                    // the other stream's last positions
-          ok = mbar_wait(&ctl.kv_full[st], phase, abort_flag);
+          ok = warp_wait(&ctl.kv_full[st], phase, abort_flag);
           if (lane == 0) mbar_arrive(&ctl.kv_empty[st]);
           ++at;
           if (++st == stages) st = 0, phase ^= 1u;
         }
-        ok = __all_sync(0xffffffffu, ok);
       }
     }
   } else {
@@ -1000,13 +999,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     auto both_streams = [&]() {                          // barrier of the eight softmax warps, bounded
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.join);
-      const bool done = mbar_wait(&ctl.join, j_uses++, abort_flag);
-      return __all_sync(0xffffffffu, done) != 0;
+      return warp_wait(&ctl.join, j_uses++, abort_flag);
     };
     for (int it = 0; ok; ++it) {
       const int islot = it & (kItems - 1);
-      ok = mbar_wait(&ctl.item_full[islot], it / kItems, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&ctl.item_full[islot], it / kItems, abort_flag);
       if (!ok) break;
       Item& o = ctl.items[islot];
       if (!o.valid) break;
@@ -1029,15 +1026,14 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
        const int kb = first + blk * kBlk, nh = khi - kb > kHalf ? 2 : 1;
        for (int h = 0; h < nh; ++h) {
         const uint32_t b = t & 1, t_sb = t_s + b * kHalf;
-        ok = mbar_wait(&ctl.s_full[s][b], t >> 1, abort_flag);
+        ok = mbar_wait(&ctl.s_full[s][b], t >> 1, abort_flag);   // voted on below, on each way
         tc_fence_after();
         if (h == 0 && (min(kb + kBlk, khi) > unit_hi || kb < unit_lo)) {
           // A weight of zero does not silence an infinite or NaN value in the product.  Such values
           // of a block that some rows attend only in part are taken out here and put back, for the
           // rows that do attend them, when the unit ends.
           const uint32_t vp = pos + ring_v(dual, blk, nblk), st = vp % stages;
-          ok = mbar_wait(&ctl.kv_full[st], vp / stages, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = __all_sync(0xffffffffu, ok) && warp_wait(&ctl.kv_full[st], vp / stages, abort_flag);
           if (!ok) break;
           uint32_t* v = reinterpret_cast<uint32_t*>(ring + st * kTileBytes);
           unsigned found = 0;
@@ -1063,6 +1059,8 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           __syncwarp();                                  // the tensor-memory instructions want whole warps
         }
         if (!any_live) {                                 // rows that nobody reads: any weights will do
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           if (lane == 0) mbar_arrive(&ctl.p_full[s][b]);
           __syncwarp();
           ++t;
@@ -1105,8 +1103,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           l *= f;
           if (blk != blk_first || h > 0) {
             // the product of the step before has to be in
-            ok = mbar_wait(&ctl.o_done[s][b ^ 1], (t - 1) >> 1, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = warp_wait(&ctl.o_done[s][b ^ 1], (t - 1) >> 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -1161,8 +1158,7 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
       // ---- the unit's (part's) result.  Dual: a thread's own row.  Single: both streams hold a share
       // of every row; stream 0 finishes dims 0-63 and stream 1 dims 64-127.
       if (blk_first < nblk) {
-        ok = mbar_wait(&ctl.o_done[s][(t - 1) & 1], (t - 1) >> 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait(&ctl.o_done[s][(t - 1) & 1], (t - 1) >> 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
       }

@@ -22,3 +22,23 @@ def test_the_kernel_fills_by_that_rule():
     groups = text[text.index("This group's positions of the unit"):text.index("own = i - n;")]
     assert "wait_to_fill(" in groups and "kv_empty" in groups
     assert not re.search(r"mbar_wait\(&ctl\.kv_empty", groups)
+
+
+def test_whole_warps_give_up_together():
+    """A wait that runs out in some lanes of a warp only must not part them: every wait of a warp that goes
+    on as one is followed by a vote.  Single lanes wait by themselves (the planning lane), and the
+    scores are waited for without a vote, which each of the three ways on from there takes first."""
+    text = KERNEL.read_text()
+    body = text[text.index("chunk_attention_kernel(const MacB200ChunkArgs"):text.index("chunk_join_kernel(")]
+    planner = body[body.index("warp == kPlanWarp && lane == 0"):body.index("the products of stream")]
+    alone = re.findall(r"\bmbar_wait\(&ctl\.(\w+)", body)
+    assert sorted(alone) == sorted(re.findall(r"\bmbar_wait\(&ctl\.(\w+)", planner) + ["s_full"])
+    steps = body[body.index("mbar_wait(&ctl.s_full"):]
+    steps = steps[:steps.index("mbar_arrive(&ctl.p_full[s][b]);\n        uint64_t sum")]
+    ways = re.split(r"if \(h == 0 &&|if \(!any_live\)|if \(__any_sync\(0xffffffffu, grow \|\| !ok\)\)", steps)
+    assert len(ways) == 4 and "break" not in ways[0] and "continue" not in ways[0]
+    for way in ways[1:]:
+        vote, leave = way.find("__all_sync(0xffffffffu, ok)"), re.search(r"\b(break|continue)\b", way)
+        assert 0 <= vote < leave.start()
+    issue = body[body.index("the products of stream"):body.index("softmax: this thread's row")]
+    assert "mbar_wait" not in issue
