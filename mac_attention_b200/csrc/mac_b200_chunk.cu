@@ -948,11 +948,12 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           if (!ok || i >= steps) return;
           const int h = i & 1;
           const uint32_t b = (t0 + i) & 1;
-          if (h == 0) {
-            st_k = next_stage();
-            if (!ok) return;
-            fence_async_smem();
-          }
+          // The weights of two steps ago lie where these scores go, and the product that reads them has
+          // another shape and accumulator: issued before, but not promised to run before.
+          ok = warp_wait(&ctl.o_done[s][b], (t0 + i + 2) >> 1, abort_flag);
+          if (h == 0) st_k = next_stage();
+          if (!ok) return;
+          fence_async_smem();
           tc_fence_after();
           const uint64_t dk = desc_k + uniform(st_k) * kDescTile + h * kDescHalf;
           if (elect_one()) {

@@ -42,3 +42,21 @@ def test_whole_warps_give_up_together():
         assert 0 <= vote < leave.start()
     issue = body[body.index("the products of stream"):body.index("softmax: this thread's row")]
     assert "mbar_wait" not in issue
+
+
+def test_scores_wait_for_the_product_that_reads_the_weights_below_them():
+    """Products of different shape and accumulator run in no promised order, so the scores of a step may be
+    written over weights only once the product of those weights is done -- also for a unit's first scores,
+    over the last unit's weights (the steps are counted through)."""
+    text = KERNEL.read_text()
+    qk = text[text.index("auto qk = [&](int i)"):]
+    qk = qk[:qk.index("__syncwarp();")]
+    wait, product = qk.find("warp_wait(&ctl.o_done[s][b], (t0 + i + 2) >> 1"), qk.find("mma_ss(")
+    assert 0 <= wait < product and "if (!ok) return;" in qk[wait:product]
+    # step n's product counts phase n / 2 of buffer n & 1; the wait of step n is for that of step n - 2,
+    # and lets the first two through, before which nothing was issued
+    for n in range(12):
+        awaited = ((n + 2) >> 1) & 1
+        before, after = (n - 2) // 2, (n - 2) // 2 + 1          # phases done without and with step n - 2
+        assert (after & 1) != awaited
+        assert n < 2 or (before & 1) == awaited
