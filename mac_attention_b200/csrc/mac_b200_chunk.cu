@@ -1049,12 +1049,19 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           if (found) {
             *reinterpret_cast<volatile unsigned*>(&o.nonfinite) = 1u;   // before any value is taken out
             __threadfence_block();
-            for (int i = 0; i < kTileBytes / 16 / 128; ++i)
-              for (int j = 0; j < 4; ++j) {
-                uint32_t& w = v[(i * 128 + r) * 4 + j];
-                if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-                if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
-              }
+#pragma unroll 1
+            for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
+              const uint32_t at = smem_u32(v + (i * 128 + r) * 4);
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                           : "r"(at)
+                           : "memory");
+              // one store a word, and the last word on it: see finite_halves()
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(finite_halves(w[0])),
+                           "r"(finite_halves(w[1])), "r"(finite_halves(w[2])), "r"(finite_halves(w[3]))
+                           : "memory");
+            }
           }
           fence_async_smem();
           __syncwarp();                                  // the tensor-memory instructions want whole warps

@@ -1,7 +1,9 @@
-// The ring of K/V blocks of the chunk attention (mac_b200_chunk.cu): its shape, and what a loading warp
-// waits for before it fills a position.  Plain C++, so that the order can be walked through on the host
-// (tests/chunk_ring_model.cpp).
+// The ring of K/V blocks of the chunk attention (mac_b200_chunk.cu): its shape, what a loading warp
+// waits for before it fills a position, and what is taken out of a block of values there.  Plain C++, so
+// that the host can walk through it (tests/chunk_ring_model.cpp).
 #pragma once
+
+#include <cstdint>
 
 #ifdef __CUDACC__
 #define MAC_RING_FN __device__ __forceinline__
@@ -34,6 +36,16 @@ struct RingShape {
 template <class Wait>
 MAC_RING_FN bool wait_to_fill(Wait&& wait) {
   return wait(true) && wait(false);
+}
+
+// A pair of bf16 values with infinities and NaN replaced by zero.  The streams of a unit of two tiles share
+// its blocks, and each takes these values out for itself before its own product, while the other's may
+// run: so a word is changed by one store, which leaves it as it stays.  Whoever stores late stores
+// what is there already.
+MAC_RING_FN uint32_t finite_halves(uint32_t w) {
+  if ((w & 0x00007f80u) == 0x00007f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+  return w;
 }
 
 }  // namespace mac_b200

@@ -60,3 +60,33 @@ def test_scores_wait_for_the_product_that_reads_the_weights_below_them():
         before, after = (n - 2) // 2, (n - 2) // 2 + 1          # phases done without and with step n - 2
         assert (after & 1) != awaited
         assert n < 2 or (before & 1) == awaited
+
+
+def test_values_are_taken_out_by_one_store_that_stands(tmp_path):
+    """A block of values that two streams share: a word with an infinity or NaN goes straight to what it stays,
+    for any two halves, and the kernel stores nothing in between."""
+    src, exe = tmp_path / "halves.cpp", tmp_path / "halves"
+    src.write_text(f"""#include <cmath>
+#include <cstring>
+#include "{KERNEL.parent / 'mac_b200_chunk_ring.h'}"
+static bool finite(uint32_t h) {{ uint32_t b = h << 16; float f; std::memcpy(&f, &b, 4); return std::isfinite(f); }}
+int main() {{
+  const uint32_t other[] = {{0u, 0x3f80u, 0x7f80u, 0xff80u, 0x7fc0u, 0xffffu, 0x7f7fu, 0x0001u, 0x8000u}};
+  for (uint32_t a = 0; a < 65536; ++a)
+    for (uint32_t b : other)
+      for (int turn = 0; turn < 2; ++turn) {{
+        const uint32_t lo = turn ? b : a, hi = turn ? a : b;
+        const uint32_t want = (finite(lo) ? lo : 0u) | (finite(hi) ? hi << 16 : 0u);
+        const uint32_t got = mac_b200::finite_halves(lo | hi << 16);
+        if (got != want || mac_b200::finite_halves(got) != got) return 1;
+      }}
+  return 0;
+}}
+""")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", str(src), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)]).returncode == 0
+    text = KERNEL.read_text()
+    out = text[text.index("if (found) {"):]
+    out = out[:out.index("fence_async_smem();")]
+    assert out.count("ld.shared") == 1 and out.count("st.shared") == 1 and out.count("finite_halves(w[") == 4
+    assert not re.search(r"\bv\[[^\]]*\]|\*v\b|&=|\|=", out)
