@@ -365,9 +365,10 @@ const char* mac_b200_last_error(void);
 int mac_b200_abi_version(void);
 
 /*
- * Reads (and clears) the sticky device status word of the current device:
- * synchronises `stream`, copies the word back, resets barrier state if a
- * bounded wait ran out.  Not on the hot path; tests and health checks poll it.
+ * Takes (reads and clears) the sticky device status word of the current device
+ * in `stream`'s order, waits for it and resets barrier state if a bounded wait
+ * ran out.  A bit is reported once: one that a kernel on another stream sets
+ * meanwhile is in this answer or in the next.  Not on the hot path; tests and health checks poll it.
  * No counterpart in the reference (its kernel has no bounded waits).
  */
 int mac_b200_query_status(uint32_t* status_out, void* stream);

@@ -1465,14 +1465,8 @@ int chunk_attention(const MacB200ChunkArgs* args, bool e4m3, void* stream_v) {
 
 }  // namespace
 
-int take_chunk_status(unsigned* bits) {
-  unsigned v = 0;
-  MAC_CUDA(cudaMemcpyFromSymbol(&v, g_chunk_status, sizeof(v)));
-  if (v != 0) {
-    const unsigned zero = 0;
-    MAC_CUDA(cudaMemcpyToSymbol(g_chunk_status, &zero, sizeof(zero)));
-  }
-  *bits = v;
+int chunk_status_word(unsigned** word) {
+  MAC_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_chunk_status));
   return MAC_B200_OK;
 }
 

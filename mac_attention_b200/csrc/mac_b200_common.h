@@ -24,16 +24,13 @@ inline int cuda_fail(cudaError_t err, const char* what) {
               cudaGetErrorName(err));
 }
 
-// Reads and clears the sticky status bits of the prefill ring-build kernels on
-// the current device (the caller has synchronised the device).
-int take_prefill_build_status(unsigned* bits);
-
-// The same for the tensor-memory variant of the sink-exclusive build.
-int take_prefill_sink_tc_status(unsigned* bits);
-
-// The same for the chunk attention and for the 8-bit pool's write and read kernels.
-int take_chunk_status(unsigned* bits);
-int take_kv8_status(unsigned* bits);
+// Where the sticky status bits of a file's kernels lie on the current device: the prefill ring build, its
+// tensor-memory variant, the chunk attention, the 8-bit pool's kernels.  mac_b200_query_status takes them
+// all in one exchange on the device.
+int prefill_build_status_word(unsigned** word);
+int prefill_sink_tc_status_word(unsigned** word);
+int chunk_status_word(unsigned** word);
+int kv8_status_word(unsigned** word);
 
 // Sink-exclusive prefill build on tcgen05 / tensor memory (validated arguments); sets
 // *launched when it ran, leaves it false when this step has to take the mma.sync kernel.

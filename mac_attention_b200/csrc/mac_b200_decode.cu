@@ -2422,25 +2422,49 @@ extern "C" int mac_b200_persistent_decode_bf16_noalloc(const MacB200DecodeArgs* 
   return launch_decode(device, p, grid, stream);
 }
 
+namespace mac_b200 {
+namespace {
+
+struct StatusWords {
+  unsigned* word[5];
+};
+// Takes the bits of every word and leaves zero, each word in one step: a bit that a kernel on another
+// stream sets meanwhile is in this answer or in the next.
+__global__ void take_status_kernel(StatusWords words, unsigned* taken) {
+  unsigned bits = 0;
+  for (int i = 0; i < 5; ++i) bits |= atomicExch(words.word[i], 0u);
+  *taken = bits;
+}
+__device__ unsigned g_taken_bits = 0;
+std::mutex g_taken_mu;   // one asker at a time: g_taken_bits holds its answer
+
+}  // namespace
+}  // namespace mac_b200
+
 extern "C" int mac_b200_query_status(uint32_t* status_out, void* stream_v) {
   MAC_REQUIRE(status_out != nullptr, "status_out must not be null");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  MAC_CUDA(cudaStreamSynchronize(stream));
-  unsigned v = 0;
-  MAC_CUDA(cudaMemcpyFromSymbol(&v, g_status, sizeof(v)));
-  unsigned build_bits = 0;
-  if (const int rc = take_prefill_build_status(&build_bits)) return rc;
-  unsigned chunk_bits = 0, kv8_bits = 0;
-  if (const int rc = take_chunk_status(&chunk_bits)) return rc;
-  if (const int rc = take_kv8_status(&kv8_bits)) return rc;
-  *status_out = v | build_bits | chunk_bits | kv8_bits;
-  if (v != 0) {
+  StatusWords words{};
+  MAC_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&words.word[0]), g_status));
+  if (const int rc = prefill_build_status_word(&words.word[1])) return rc;
+  if (const int rc = prefill_sink_tc_status_word(&words.word[2])) return rc;
+  if (const int rc = chunk_status_word(&words.word[3])) return rc;
+  if (const int rc = kv8_status_word(&words.word[4])) return rc;
+  unsigned* taken = nullptr;
+  MAC_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&taken), g_taken_bits));
+  unsigned bits = 0;
+  {
+    std::lock_guard<std::mutex> lock(g_taken_mu);
+    take_status_kernel<<<1, 1, 0, stream>>>(words, taken);
+    MAC_CUDA(cudaGetLastError());
+    MAC_CUDA(cudaMemcpyAsync(&bits, taken, sizeof(bits), cudaMemcpyDeviceToHost, stream));
+    MAC_CUDA(cudaStreamSynchronize(stream));
+  }
+  *status_out = bits;
+  if (bits & MAC_B200_STATUS_BARRIER_TIMEOUT) {
     const unsigned zero = 0;
     MAC_CUDA(cudaDeviceSynchronize());
-    MAC_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
-    if (v & MAC_B200_STATUS_BARRIER_TIMEOUT) {
-      MAC_CUDA(cudaMemcpyToSymbol(g_bar_count, &zero, sizeof(zero)));
-    }
+    MAC_CUDA(cudaMemcpyToSymbol(g_bar_count, &zero, sizeof(zero)));
   }
   return MAC_B200_OK;
 }

@@ -217,14 +217,8 @@ unsigned blocks_for(int64_t tasks) {
 
 }  // namespace
 
-int take_kv8_status(unsigned* bits) {
-  unsigned v = 0;
-  MAC_CUDA(cudaMemcpyFromSymbol(&v, g_kv8_status, sizeof(v)));
-  if (v != 0) {
-    const unsigned zero = 0;
-    MAC_CUDA(cudaMemcpyToSymbol(g_kv8_status, &zero, sizeof(zero)));
-  }
-  *bits = v;
+int kv8_status_word(unsigned** word) {
+  MAC_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_kv8_status));
   return MAC_B200_OK;
 }
 

@@ -640,16 +640,8 @@ __global__ void prefill_build_finish_kernel(const MacB200PrefillBuildArgs a) {
 
 }  // namespace
 
-int take_prefill_build_status(unsigned* bits) {
-  unsigned v = 0;
-  MAC_CUDA(cudaMemcpyFromSymbol(&v, g_build_status, sizeof(v)));
-  if (v != 0) {
-    const unsigned zero = 0;
-    MAC_CUDA(cudaMemcpyToSymbol(g_build_status, &zero, sizeof(zero)));
-  }
-  unsigned tc = 0;
-  if (const int rc = take_prefill_sink_tc_status(&tc)) return rc;
-  *bits = v | tc;
+int prefill_build_status_word(unsigned** word) {
+  MAC_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_build_status));
   return MAC_B200_OK;
 }
 

@@ -645,14 +645,8 @@ TcEncodeTiledFn tc_encode_tiled_fn() {
 
 }  // namespace
 
-int take_prefill_sink_tc_status(unsigned* bits) {
-  unsigned v = 0;
-  MAC_CUDA(cudaMemcpyFromSymbol(&v, g_tc_status, sizeof(v)));
-  if (v != 0) {
-    const unsigned zero = 0;
-    MAC_CUDA(cudaMemcpyToSymbol(g_tc_status, &zero, sizeof(zero)));
-  }
-  *bits = v;
+int prefill_sink_tc_status_word(unsigned** word) {
+  MAC_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_tc_status));
   return MAC_B200_OK;
 }
 
