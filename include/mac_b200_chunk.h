@@ -36,6 +36,8 @@ extern "C" {
  *     out = sum_j softmax_j(sm_scale * q.k_j) v_j,   lse = ln sum_j exp(sm_scale * q.k_j)
  * A row that attends nothing (p < 0, window 0) gets out = 0, lse = -inf.  A
  * value that a row does not attend does not reach it, whatever it holds.
+ * Weights are summed before they are normalised, in fp32 and up to 2^8 each:
+ * out may be infinite or NaN where |v| * attended keys * 2^8 passes the fp32 range.
  *
  * Rows of q outside [offsets[0], offsets[B]) reach nothing and are not written
  * in out / lse.  q and out must not share memory.  All lengths are read on the device; nothing about a call has to
