@@ -21,7 +21,9 @@
 //   the last eight   softmax streams 0 and 1, a thread a row: scores from tensor memory, running
 //                    maximum and sum in fp32, bf16 weights back over the scores, results out
 //   warps 0, 1       issue the streams' products: S = Q K^T from shared memory, O += P V with P from
-//                    tensor memory and V from the rows as they lie in the pool (keys x dims)
+//                    tensor memory and V from the rows as they lie in the pool (keys x dims); products
+//                    that differ in shape are not promised to run in the order of issue, so where one
+//                    writes what another reads it is issued after that one is done
 //   warps 4-7 (-15)  fetch K/V rows by the page table into the swizzled operand layout (cp.async; the
 //                    8-bit pool's rows by way of a raw buffer, widened to bf16)
 //   warp 2           works out the units of this CTA's part, fetches the query tiles
@@ -31,20 +33,23 @@
 // is rare, and exact when it happens.  Weights are rounded to bf16 for the second product (the
 // operand type); the sum of weights is taken before that rounding, in fp32.
 //
-// Measured (B200: 6564 GB/s copied, 1675 TFLOP/s of a bf16 product):
-//   decode, 16 requests x 32768 tokens, 32 / 8 heads: 323 us back to back, 0.98 of the copy rate (390
-//     with cold caches); the 8-bit pool 349 (392) us, 0.46 (0.41): no one part bounds it (without
-//     the widening's stores 0.92 of the time, without the row fetches 0.96, without the softmax 0.93),
-//     the chain through the ring's few positions does
-//   prompt, 4096 tokens behind 28672 cached, 32 / 8 heads: 2.30 ms, 897 TFLOP/s; 2 x 1024 tokens of
-//     8192 over the 8-bit pool 555 us, 840 TFLOP/s.  Without the softmax's arithmetic such a call
+// Measured (B200: 6564 GB/s copied, 1675 TFLOP/s of a bf16 product; calls on inputs that change from call
+// to call, here and below, unless it says otherwise):
+//   decode, 16 requests x 30000-32768 tokens, 32 / 8 heads: 392-399 us, 0.80 of the copy rate (the same
+//     call over and over 338, 0.94); the 8-bit pool 389-398 us, 0.40 (353-370, 0.44): no one part bounds
+//     it (without the widening's stores 0.92 of the time, without the row fetches 0.96, without the
+//     softmax 0.93), the chain through the ring's few positions does
+//   prompt, 4096 tokens behind 28672 cached, 32 / 8 heads: 2285-2319 us, 889-902 TFLOP/s; 2 x 1024 tokens
+//     of 8192 over the 8-bit pool 545-554 us, 841-854 TFLOP/s.  Without the softmax's arithmetic such a call
 //     still takes 0.85 of its time: a product of 128 x 64 from shared memory is bound by the reads
 //     of its operands (412 cycles for 256 of arithmetic) and the hand-overs between the products
 //     and the softmax are not hidden entirely.  ncu (1024 tokens of 8192, 64 / 8 heads): tensor cores
-//     46 %, issue slots 44 %, exponentials 46 % of the cycles.
-//   8 prompts of 2048 in a band of 1024: 576 us, 632 TFLOP/s (masked halves of blocks count as none)
-//   three requests of drafted tokens behind 1000: 22 us a call by itself; a single token 11 us, of
-//     which 3 are set-up (lengths, tensor memory) and 5 the chain of one block's steps
+//     46 %, issue slots 45 %, exponentials 46 % of the cycles.
+//   8 prompts of 1500-2048 in a band of 1024: 564-573 us, 634-645 TFLOP/s (masked halves of blocks count
+//     as none)
+//   three requests of drafted tokens behind 1000: 22 us a call by itself; a single token of 128, calls in
+//     a row within one graph, 11.4 us, of which 3 are set-up (lengths, tensor memory) and 5 the chain of
+//     one block's steps
 // No gain, measured on the same calls: steps of 128 keys, one warp that issues for both streams,
 // turns between the streams' products, two threads a row, a quarter of the exponentials by a
 // polynomial, bulk row gathers instead of cp.async (80 cycles each to issue).
@@ -498,8 +503,9 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
                         ((b == b0 ? mine0 : load_request(a, b, blockIdx.x == 0)).n + tile_tokens - 1) / tile_tokens);
   // pairs of tiles once there are enough of them for every CTA
   const int span = scan_cta<kThreads>(mine, before, ctl.scan) >= 2ll * gridDim.x ? 2 * tile_tokens : tile_tokens;
-  // The 8-bit pool's ring is short.  Where every unit is of one tile the second query buffer, in front of
-  // it, joins it (decode 403 -> 392 us; a sixth position of bf16 gains nothing: 391 either way).
+  // The 8-bit pool's ring is short: three positions.  Where every unit is of one tile the second query
+  // buffer, in front of it, joins it as a fourth (decode 390 us, 405 with three; a sixth position of
+  // bf16 gains nothing).  Four are no multiple of the three groups that fill them: see wait_to_fill().
   const int stages = span == tile_tokens ? kStages + RingShape<kE4m3>::kSpare : kStages;
   uint8_t* const ring = smem + kSmemKv - (stages - kStages) * kTileBytes;
   long long units = 0;
@@ -583,8 +589,8 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
     // e4m3: eight lanes a row, into a raw buffer ahead of time (48 KB of them; held in registers the rows
     // were waited for all at once), then widened to bf16 with their scales on the way into the operand
     // layout.  The widened rows are exact: from there on the two pools go the same way.  Four warps
-    // take every third position, so three are widened at once (eight warps on one after the other:
-    // 430 us for the decode call above, 398 this way).
+    // take every third position, so three are widened at once (eight warps on one after the other: 8 %
+    // more for the decode call above).
     constexpr int kLanes = kE4m3 ? 8 : 16;               // of a row
     const int sub = lane / kLanes, c = lane % kLanes;    // row of a load, 16 bytes of it
     const int64_t row_stride = static_cast<int64_t>(a.Hkv) * (kE4m3 ? 128 : 256);
@@ -969,10 +975,11 @@ chunk_attention_kernel(const MacB200ChunkArgs a, const __grid_constant__ CUtenso
           __syncwarp();
         };
         if (kE4m3 && !dual) {
-          // Where the ring is as short as three positions and the streams alternate, both products of a
-          // block's values come before the scores of the stream's next block: values that wait for the
-          // next keys before they are given back hold up the keys behind them.  (Decode of 16 x 32000
-          // tokens 370 us, 441 in the other order; five positions of bf16 gain nothing by it.)
+          // Where the ring is short (three positions, four in a call whose units are all of one tile) and
+          // the streams alternate, both products of a block's values come before the scores of the
+          // stream's next block: values that wait for the next keys before they are given back hold up
+          // the keys behind them.  (The decode call above, four positions: 390 us, 401 in the other
+          // order; five positions of bf16 gain nothing by it, 397 us either way.)
           for (int i = 0; ok && steps > 0 && i < steps + 2; i += 2) pv(i - 2), pv(i - 1), qk(i), qk(i + 1);
         } else {
           for (int i = 0; ok && steps > 0 && i < steps + 2; ++i) pv(i - 2), qk(i);

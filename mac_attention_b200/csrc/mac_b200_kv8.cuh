@@ -42,8 +42,9 @@ __device__ __forceinline__ float2 kv8_unpack2(uint32_t codes) {
 }
 
 // 32 bytes: one store of a whole sector where the address allows it, since half a sector costs the memory
-// system as much (chunk attention, 8 prompts of 2048 in a band of 1024: 576 us, 605 with 16-byte
-// stores, 547 with none; 100000 rows read back from the 8-bit pool: 101 us, 109).
+// system as much (measured in turn: chunk attention, 8 prompts of 1500-2048 in a band of 1024, 5 % less
+// than with 16-byte stores, and 5 % less again with none; 100000 rows read back from the 8-bit pool 101 us
+// instead of 109).
 __device__ __forceinline__ void store32(uint4* dst, const uint32_t (&w)[8], bool aligned32) {
   if (aligned32) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
